@@ -74,6 +74,33 @@ class EpPeers(Structure):
                 ("ret", c_void_p * EP_MAX_RANKS)]
 
 
+class RouteDesc(Structure):
+    """Mirror of ``ag_route_desc_t``."""
+
+    _fields_ = [("logits", c_void_p), ("ld", c_int64), ("bias", c_void_p), ("rows_used", c_void_p), ("ids", c_void_p), ("weights", c_void_p),
+                ("tokens", c_int64), ("dtype", c_int32), ("experts", c_int32), ("top_k", c_int32), ("groups", c_int32), ("top_groups", c_int32),
+                ("scoring", c_int32), ("group_max", c_int32), ("renormalize", c_int32), ("scale", c_float), ("stream", c_void_p)]
+
+
+class RouteLayoutDesc(Structure):
+    """Mirror of ``ag_route_layout_desc_t``."""
+
+    _fields_ = [("ids", c_void_p), ("ids_64", c_int32), ("top_k", c_int32), ("tokens", c_int64), ("experts", c_int32), ("alignment", c_int32),
+                ("max_rows", c_int32), ("rows", c_int64), ("pair_row", c_void_p), ("row_token", c_void_p), ("rows_per_expert", c_void_p),
+                ("offsets", c_void_p), ("expert_list", c_void_p), ("masked_m", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_uint64),
+                ("status", c_void_p), ("stream", c_void_p)]
+
+
+class LinearDesc(Structure):
+    """Mirror of ``ag_linear_desc_t``."""
+
+    _fields_ = ([(f, c_int32) for f in ("dtype", "out_dtype", "bias_dtype", "activation")] + [(f, c_int64) for f in ("m", "n", "k")]
+                + [(f, c_void_p) for f in ("x", "weight", "bias", "residual", "y", "pre")]
+                + [(f, c_int64) for f in ("ldx", "ldw", "ldr", "ldy", "ldp")] + [("dy", c_void_p), ("lddy", c_int64)]
+                + [(f, c_void_p) for f in ("dx", "dweight", "dbias", "workspace")]
+                + [("workspace_bytes", c_uint64), ("status", c_void_p), ("timeout_ms", c_uint32), ("stream", c_void_p)])
+
+
 EXPORTS = [
     "ag_m_grouped_bf16_gemm_nt",
     "ag_m_grouped_fp8_gemm_nt",
@@ -120,6 +147,15 @@ EXPORTS = [
     "ag_quant_rows_int8",
     "ag_silu_mul_quant_int8",
     "ag_combine_topk_f32",
+    "ag_route_topk",
+    "ag_route_topk_backward",
+    "ag_route_layout",
+    "ag_route_layout_workspace_bytes",
+    "ag_combine_topk_backward",
+    "ag_linear",
+    "ag_linear_backward",
+    "ag_linear_backward_workspace_bytes",
+    "ag_linear_desc_size",
     "ag_gemm_desc_size",
     "ag_last_error",
     "ag_version",
@@ -204,6 +240,25 @@ def load() -> ctypes.CDLL:
     lib.ag_silu_mul_quant_int8.restype = c_int32
     lib.ag_combine_topk_f32.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p]
     lib.ag_combine_topk_f32.restype = c_int32
+    lib.ag_route_topk.argtypes = [POINTER(RouteDesc)]
+    lib.ag_route_topk.restype = c_int32
+    lib.ag_route_topk_backward.argtypes = [c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_float,
+                                           c_void_p, c_void_p]
+    lib.ag_route_topk_backward.restype = c_int32
+    lib.ag_route_layout.argtypes = [POINTER(RouteLayoutDesc)]
+    lib.ag_route_layout.restype = c_int32
+    lib.ag_route_layout_workspace_bytes.argtypes = [c_int64, c_int32]
+    lib.ag_route_layout_workspace_bytes.restype = c_uint64
+    lib.ag_combine_topk_backward.argtypes = [c_void_p, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_void_p]
+    lib.ag_combine_topk_backward.restype = c_int32
+    for name in ("ag_linear", "ag_linear_backward"):
+        getattr(lib, name).argtypes = [POINTER(LinearDesc)]
+        getattr(lib, name).restype = c_int32
+    lib.ag_linear_backward_workspace_bytes.argtypes = [POINTER(LinearDesc)]
+    lib.ag_linear_backward_workspace_bytes.restype = c_uint64
+    lib.ag_linear_desc_size.argtypes = []
+    lib.ag_linear_desc_size.restype = c_uint64
     lib.ag_selftest_wait_limit.argtypes = [c_uint32, c_void_p, c_void_p]
     lib.ag_selftest_wait_limit.restype = c_int32
     lib.ag_probe_mma_issue.argtypes = [c_int32, c_int32, c_int32, ctypes.POINTER(ctypes.c_double)]

@@ -416,6 +416,7 @@ const char* status_text(int code) {
     case agb::ST_TIMEOUT_PROBE: return "wait-limit self test expired (expected)";
     case AG_EP_BAD_EXPERT: return "the routing names an expert id outside [0, num_experts)";
     case AG_EP_OVERFLOW: return "a rank's experts received more rows than its exchange buffers hold";
+    case AG_COMBINE_ROW_TWICE: return "two (token, slot) pairs of a combine gradient name the same row";
     default: return "unknown status";
   }
 }
@@ -441,6 +442,25 @@ int scratch_need(int kind, const ag_gemm_desc_t* g, uint64_t* out) {
 int agb_run_desc(int kind, const ag_gemm_desc_t* desc) { return run(kind, desc); }
 int agb_scratch_need(int kind, const ag_gemm_desc_t* desc, uint64_t* out) { return scratch_need(kind, desc, out); }
 int agb_fail(int code, const char* message) { return fail(code, "%s", message); }
+int agb_device_sm_count(int* out) { return device_sm_count(out); }
+int32_t* agb_default_status_word() { return default_status_word(); }
+// 2-D map of 16-bit elements with the 128-byte swizzle: rows of `inner` elements `pitch_bytes` apart, boxes of 64 elements x
+// `box_rows` rows; what lies outside reads as zero.
+int agb_encode_16bit_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch_bytes, uint32_t box_rows,
+                        const char* what) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return fail(AG_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t gdim[2] = {inner, rows};
+  cuuint64_t gstr[1] = {pitch_bytes};
+  cuuint32_t box[2] = {64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(AG_E_CUDA, "cuTensorMapEncodeTiled failed for %s (CUresult %d; base %p, %llu x %llu, pitch %llu)", what, static_cast<int>(r), base,
+                static_cast<unsigned long long>(rows), static_cast<unsigned long long>(inner), static_cast<unsigned long long>(pitch_bytes));
+  return AG_OK;
+}
 
 extern "C" {
 

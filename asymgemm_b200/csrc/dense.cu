@@ -1,0 +1,380 @@
+// Dense products of the layer around the grouped GEMMs (router logits, shared experts, projections): y = act(x W^T + b) + r and
+// its gradients. Operands bf16 or fp16, fp32 accumulation, output in the operands' type or fp32; see dense_kernel.cuh.
+#include "dense_kernel.cuh"
+
+#include "../../include/asymgemm_b200.h"
+
+int agb_fail(int code, const char* message);
+int agb_device_sm_count(int* out);
+int32_t* agb_default_status_word();
+int agb_encode_16bit_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch_bytes, uint32_t box_rows, const char* what);
+
+namespace agb {
+
+// ------------------------------------------------------------------------------------------------ gradient before the activation
+// dz = dy * act'(z), rounded to the operands' type because the tensor core takes it as an operand of the two products that
+// follow (half a step of that type per element, like the operands themselves), with rows padded to 16 bytes; and, in the
+// same pass over dy, the column sums of the unrounded dz that make the bias gradient. A thread owns columns and walks rows,
+// so the sums are fp32 additions in a fixed order: per block of rows here, over the blocks in column_sums_kernel.
+// Bound by memory: dy and z are read once, dz is written once.
+constexpr int kDzCols = 256, kDzThreads = 256;
+
+__device__ __forceinline__ float slope(float z, int act) {
+  if (act == ACT_RELU) return z > 0.f ? 1.f : z != z ? z : 0.f;
+  if (act == ACT_GELU) return normcdff(z) + z * 0.39894228f * expf(-0.5f * z * z);
+  if (act == ACT_SILU) {
+    const float s = 1.f / (1.f + expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  return 1.f;
+}
+
+struct DzParams {
+  const void* dy;
+  const void* pre;
+  void* dz;             // or null: only the sums are wanted
+  float* partial;       // [row blocks, n] or null
+  long long m, n, ld_dy, ld_pre, ld_dz;
+  int dy_type, type, act, rows_per_block;
+};
+
+template <int V>   // 8: 16-byte pieces of 16-bit rows; 1: any alignment
+__global__ void __launch_bounds__(kDzThreads) dz_kernel(const DzParams p) {
+  __shared__ float sums[8][kDzCols];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long r0 = static_cast<long long>(blockIdx.y) * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.m);
+  float acc[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  // columns of this thread: V consecutive ones, or every 32nd
+  auto column = [&](int i) { return static_cast<long long>(blockIdx.x) * kDzCols + (V == 8 ? tx * 8 + i : tx + 32 * i); };
+  for (long long r = r0 + ty; r < r1; r += 8) {
+    float g[8], z[8];
+    if constexpr (V == 8) {
+      const long long c = column(0);
+      if (c >= p.n) break;
+      if (p.dy_type == T_FP32) {
+        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.dy) + r * p.ld_dy + c);
+        const float4 a = src[0], b = src[1];
+        g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w; g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+      } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dy) + r * p.ld_dy + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = load_as_float(&u, i, p.dy_type);
+      }
+      if (p.act != ACT_NONE) {
+        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.pre) + r * p.ld_pre + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = load_as_float(&u, i, p.type);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long c = column(i);
+        g[i] = c < p.n ? load_as_float(p.dy, r * p.ld_dy + c, p.dy_type) : 0.f;
+        z[i] = c < p.n && p.act != ACT_NONE ? load_as_float(p.pre, r * p.ld_pre + c, p.type) : 0.f;
+      }
+    }
+    if (p.act != ACT_NONE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] *= slope(z[i], p.act);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += g[i];
+    if (p.dz != nullptr) {
+      if constexpr (V == 8) {
+        uint4 u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_from_float(&u, i, p.type, g[i]);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dz) + r * p.ld_dz + column(0)) = u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (column(i) < p.n) store_from_float(p.dz, r * p.ld_dz + column(i), p.type, g[i]);
+      }
+    }
+  }
+  if (p.partial == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[ty][V == 8 ? tx * 8 + i : tx + 32 * i] = acc[i];
+  __syncthreads();
+  const long long c = static_cast<long long>(blockIdx.x) * kDzCols + threadIdx.x;
+  if (c >= p.n) return;
+  float s = 0.f;
+#pragma unroll
+  for (int y = 0; y < 8; ++y) s += sums[y][threadIdx.x];
+  p.partial[blockIdx.y * p.n + c] = s;
+}
+
+// out[c] = sum over the row blocks of partial[., c]; 32 columns x 8 interleaved shares of the blocks per CTA, joined in order.
+__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, long long blocks, long long n, void* out, int type) {
+  __shared__ float sums[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long c = static_cast<long long>(blockIdx.x) * 32 + tx;
+  float s = 0.f;
+  if (c < n)
+    for (long long b = ty; b < blocks; b += 8) s += partial[b * n + c];
+  sums[ty][tx] = s;
+  __syncthreads();
+  if (ty != 0 || c >= n) return;
+#pragma unroll
+  for (int y = 1; y < 8; ++y) s += sums[y][tx];
+  store_from_float(out, c, type, s);
+}
+
+}  // namespace agb
+
+namespace {
+
+bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// An operand of a product: element (row, k) at p[row * ld + k], or, MN-major, at p[k * ld + row].
+struct Operand {
+  const void* p;
+  int64_t ld, rows;
+  bool mn;
+  const char* what;
+};
+
+struct Plan {
+  int bn, splits;
+  bool swapped;
+};
+
+// Tile and split of a product. The narrower side is B, so that little of a tile is padding and the long side's rows (the
+// weights of a decode step) are spread over as many CTAs as possible; the contraction is split while the grid stays within
+// the CTAs that are resident at once and every split keeps four steps.
+Plan plan_product(const Operand& a, const Operand& b, int64_t steps, int sms) {
+  Plan pl{};
+  // the MN-major tile kernel exists for A alone, or for both
+  pl.swapped = a.mn == b.mn ? (!a.mn && a.rows <= 64 && b.rows > a.rows) : b.mn;
+  const int64_t ra = pl.swapped ? b.rows : a.rows, rb = pl.swapped ? a.rows : b.rows;
+  const bool both = a.mn && b.mn;
+  auto tiles = [&](int bn) { return (ra + agb::kTileA - 1) / agb::kTileA * ((rb + bn - 1) / bn); };
+  if (!both && rb <= 16) pl.bn = 16;
+  else if (!both && rb <= 32) pl.bn = 32;
+  else pl.bn = rb > 64 && tiles(128) >= sms ? 128 : 64;
+  const int64_t room = pl.bn == 128 ? sms : 2 * sms;
+  pl.splits = 1;
+  while (pl.splits < 8 && tiles(pl.bn) * pl.splits * 2 <= room && steps >= pl.splits * 2 * 4) pl.splits *= 2;
+  return pl;
+}
+
+template <int BN, bool A_MN, bool B_MN>
+cudaError_t launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, cudaStream_t stream) {
+  using L = agb::TileSmem<BN>;
+  static_assert(L::dyn_bytes * (BN >= 128 ? 1 : 2) <= 232448, "tile configuration does not fit in shared memory");
+  auto kernel = agb::dense_tile_kernel<BN, A_MN, B_MN>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::dyn_bytes);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int64_t tiles = (static_cast<int64_t>(p.rows_a) + agb::kTileA - 1) / agb::kTileA * p.tiles_b;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(agb::kTileThreads);
+  cfg.dynamicSmemBytes = L::dyn_bytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p, splits);
+}
+
+// What goes into the epilogue; the rest of DenseParams follows from the operands.
+int run_product(Operand a, Operand b, int64_t k, int type, agb::DenseParams p, cudaStream_t stream) {
+  int sms = 0;
+  if (int rc = agb_device_sm_count(&sms)) return rc;
+  const int64_t steps = (k + agb::kStepK - 1) / agb::kStepK;
+  const Plan pl = plan_product(a, b, steps, sms);
+  if (pl.swapped) {
+    const Operand t = a;
+    a = b;
+    b = t;
+  }
+  CUtensorMap ma, mb;
+  auto encode = [&](CUtensorMap* map, const Operand& o, int tile_rows) {
+    return o.mn ? agb_encode_16bit_2d(map, o.p, static_cast<uint64_t>(o.rows), static_cast<uint64_t>(k), static_cast<uint64_t>(o.ld) * 2, agb::kStepK, o.what)
+                : agb_encode_16bit_2d(map, o.p, static_cast<uint64_t>(k), static_cast<uint64_t>(o.rows), static_cast<uint64_t>(o.ld) * 2,
+                                      static_cast<uint32_t>(tile_rows), o.what);
+  };
+  if (int rc = encode(&ma, a, agb::kTileA)) return rc;
+  if (int rc = encode(&mb, b, pl.bn)) return rc;
+  p.rows_a = static_cast<int>(a.rows);
+  p.rows_b = static_cast<int>(b.rows);
+  p.steps = static_cast<int>(steps);
+  p.tiles_b = static_cast<int>((b.rows + pl.bn - 1) / pl.bn);
+  p.swapped = pl.swapped;
+  // operand format 0 = fp16, 1 = bf16; bits 15 and 16: A, B are MN-major
+  p.idesc = agb::make_idesc(1, type == AG_T_BF16 ? 1u : 0u, static_cast<uint32_t>(pl.bn)) | (a.mn ? 1u << 15 : 0u) | (b.mn ? 1u << 16 : 0u);
+  cudaError_t e = cudaErrorInvalidValue;
+  if (!a.mn && !b.mn) {
+    if (pl.bn == 16) e = launch_tile<16, false, false>(ma, mb, p, pl.splits, stream);
+    else if (pl.bn == 32) e = launch_tile<32, false, false>(ma, mb, p, pl.splits, stream);
+    else if (pl.bn == 64) e = launch_tile<64, false, false>(ma, mb, p, pl.splits, stream);
+    else e = launch_tile<128, false, false>(ma, mb, p, pl.splits, stream);
+  } else if (!b.mn) {
+    if (pl.bn == 16) e = launch_tile<16, true, false>(ma, mb, p, pl.splits, stream);
+    else if (pl.bn == 32) e = launch_tile<32, true, false>(ma, mb, p, pl.splits, stream);
+    else if (pl.bn == 64) e = launch_tile<64, true, false>(ma, mb, p, pl.splits, stream);
+    else e = launch_tile<128, true, false>(ma, mb, p, pl.splits, stream);
+  } else {
+    if (pl.bn == 64) e = launch_tile<64, true, true>(ma, mb, p, pl.splits, stream);
+    else e = launch_tile<128, true, true>(ma, mb, p, pl.splits, stream);
+  }
+  return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+}
+
+int size_of(int type) { return type == AG_T_FP32 ? 4 : 2; }
+
+int check_common(const ag_linear_desc_t* g) {
+  if (g == nullptr) return agb_fail(AG_E_INVALID, "desc is NULL");
+  if (g->dtype != AG_T_BF16 && g->dtype != AG_T_FP16) return agb_fail(AG_E_INVALID, "x and weight must be bf16 or fp16");
+  if (g->out_dtype != g->dtype && g->out_dtype != AG_T_FP32) return agb_fail(AG_E_INVALID, "the output is of the operands' type or fp32");
+  if (g->bias_dtype != g->dtype && g->bias_dtype != AG_T_FP32) return agb_fail(AG_E_INVALID, "the bias is of the operands' type or fp32");
+  if (g->activation < AG_ACT_NONE || g->activation > AG_ACT_SILU) return agb_fail(AG_E_INVALID, "unknown activation");
+  if (g->m < 0 || g->n <= 0 || g->k <= 0 || g->m > 0x7fffff00LL || g->n > 0x7fffff00LL || g->k > 0x7fffff00LL) return agb_fail(AG_E_INVALID, "bad sizes");
+  if (g->k % 8 != 0) return agb_fail(AG_E_INVALID, "k must be a multiple of 8 (16-byte rows)");
+  if (g->ldw < g->k || g->ldw % 8 != 0 || (g->m > 0 && (g->ldx < g->k || g->ldx % 8 != 0)))
+    return agb_fail(AG_E_INVALID, "rows of x and weight must start on 16-byte boundaries and not overlap");
+  if (!aligned_to(g->x, 16) || !aligned_to(g->weight, 16)) return agb_fail(AG_E_INVALID, "x and weight must be 16-byte aligned");
+  return AG_OK;
+}
+
+// How the gradient before the activation is had: as dy itself where the products can take that, else from dz_kernel.
+bool needs_dz(const ag_linear_desc_t* g) {
+  return g->activation != AG_ACT_NONE || g->out_dtype != g->dtype || g->lddy % 8 != 0 || !aligned_to(g->dy, 16);
+}
+int64_t dz_ld(const ag_linear_desc_t* g) { return (g->n + 7) / 8 * 8; }
+// Rows per block of dz_kernel: enough blocks to fill the GPU a few times, and no more partial sums than 512 blocks make.
+int64_t dz_rows(const ag_linear_desc_t* g) {
+  const int64_t col_blocks = (g->n + agb::kDzCols - 1) / agb::kDzCols;
+  int64_t rows = (g->m * col_blocks + 1183) / 1184;
+  if (rows < (g->m + 511) / 512) rows = (g->m + 511) / 512;
+  return (rows < 8 ? 8 : rows + 7) / 8 * 8;
+}
+uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
+struct BackwardSpace {
+  uint64_t dz, partial, total;
+};
+BackwardSpace backward_space(const ag_linear_desc_t* g) {
+  BackwardSpace s{};
+  if (needs_dz(g) && (g->dx != nullptr || g->dweight != nullptr)) s.dz = align256(static_cast<uint64_t>(g->m) * dz_ld(g) * 2);
+  if (g->dbias != nullptr) s.partial = align256(static_cast<uint64_t>((g->m + dz_rows(g) - 1) / dz_rows(g)) * g->n * 4);
+  s.total = s.dz + s.partial;
+  return s;
+}
+
+agb::DenseParams plain_output(const ag_linear_desc_t* g, void* out, int64_t ld, int type) {
+  agb::DenseParams p{};
+  p.out = out;
+  p.ldo = ld;
+  p.out_type = type;
+  p.status = g->status != nullptr ? g->status : agb_default_status_word();
+  p.timeout_ns = static_cast<unsigned long long>(g->timeout_ms ? g->timeout_ms : 4000u) * 1000000ull;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t ag_linear_desc_size(void) { return sizeof(ag_linear_desc_t); }
+
+int ag_linear(const ag_linear_desc_t* g) {
+  if (int rc = check_common(g)) return rc;
+  if (g->m == 0) return AG_OK;
+  if (g->x == nullptr || g->weight == nullptr || g->y == nullptr) return agb_fail(AG_E_INVALID, "x, weight and y must be non-NULL");
+  const int out_size = size_of(g->out_dtype);
+  if (g->ldy < g->n || (g->residual != nullptr && g->ldr < g->n) || (g->pre != nullptr && g->ldp < g->n))
+    return agb_fail(AG_E_INVALID, "rows of y, residual and pre must not overlap");
+  if (!aligned_to(g->y, out_size) || !aligned_to(g->residual, out_size) || !aligned_to(g->pre, 2) || !aligned_to(g->bias, size_of(g->bias_dtype)))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  agb::DenseParams p = plain_output(g, g->y, g->ldy, g->out_dtype);
+  if (p.status == nullptr) return agb_fail(AG_E_CUDA, "no status word");
+  p.bias = g->bias;
+  p.bias_type = g->bias_dtype;
+  p.residual = g->residual;
+  p.ldr = g->ldr;
+  p.pre = g->pre;
+  p.ldp = g->ldp;
+  p.pre_type = g->dtype;
+  p.act = g->activation;
+  return run_product({g->x, g->ldx, g->m, false, "x"}, {g->weight, g->ldw, g->n, false, "weight"}, g->k, g->dtype, p,
+                     static_cast<cudaStream_t>(g->stream));
+}
+
+uint64_t ag_linear_backward_workspace_bytes(const ag_linear_desc_t* g) { return g == nullptr || g->m <= 0 || g->n <= 0 ? 0 : backward_space(g).total; }
+
+int ag_linear_backward(const ag_linear_desc_t* g) {
+  if (int rc = check_common(g)) return rc;
+  if (g->dx == nullptr && g->dweight == nullptr && g->dbias == nullptr) return AG_OK;
+  cudaStream_t stream = static_cast<cudaStream_t>(g->stream);
+  if (!aligned_to(g->dbias, size_of(g->bias_dtype)) || !aligned_to(g->dx, 2) || !aligned_to(g->dweight, 2))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  if (g->m == 0) {      // a sum over no rows
+    cudaError_t e = cudaSuccess;
+    if (g->dweight != nullptr) e = cudaMemsetAsync(g->dweight, 0, static_cast<size_t>(g->n) * g->k * 2, stream);
+    if (e == cudaSuccess && g->dbias != nullptr) e = cudaMemsetAsync(g->dbias, 0, static_cast<size_t>(g->n) * size_of(g->bias_dtype), stream);
+    return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+  }
+  if (g->x == nullptr || g->weight == nullptr || g->dy == nullptr) return agb_fail(AG_E_INVALID, "x, weight and dy must be non-NULL");
+  if (g->activation != AG_ACT_NONE && g->pre == nullptr) return agb_fail(AG_E_INVALID, "the gradient of an activation wants `pre` of the forward call");
+  if (g->lddy < g->n || (g->pre != nullptr && g->ldp < g->n)) return agb_fail(AG_E_INVALID, "rows of dy and pre must not overlap");
+  if (!aligned_to(g->dy, size_of(g->out_dtype)) || !aligned_to(g->pre, 2)) return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  const BackwardSpace space = backward_space(g);
+  if (space.total > 0 && (g->workspace == nullptr || g->workspace_bytes < space.total || !aligned_to(g->workspace, 256)))
+    return agb_fail(AG_E_INVALID, "workspace too small or not 256-byte aligned (ag_linear_backward_workspace_bytes)");
+
+  const void* dz = g->dy;
+  int64_t ld = g->lddy;
+  if (space.dz > 0 || space.partial > 0) {
+    agb::DzParams p{};
+    p.dy = g->dy;
+    p.pre = g->pre;
+    p.m = g->m;
+    p.n = g->n;
+    p.ld_dy = g->lddy;
+    p.ld_pre = g->ldp;
+    p.dy_type = g->out_dtype;
+    p.type = g->dtype;
+    p.act = g->activation;
+    p.rows_per_block = static_cast<int>(dz_rows(g));
+    if (space.dz > 0) {
+      dz = p.dz = g->workspace;
+      ld = p.ld_dz = dz_ld(g);
+    }
+    if (space.partial > 0) p.partial = reinterpret_cast<float*>(static_cast<char*>(g->workspace) + space.dz);
+    const int64_t blocks = (g->m + p.rows_per_block - 1) / p.rows_per_block;
+    const bool wide = g->n % 8 == 0 && aligned_to(g->dy, 16) && g->lddy * size_of(g->out_dtype) % 16 == 0 &&
+                      (g->activation == AG_ACT_NONE || (aligned_to(g->pre, 16) && g->ldp % 8 == 0));
+    const dim3 grid(static_cast<unsigned>((g->n + agb::kDzCols - 1) / agb::kDzCols), static_cast<unsigned>(blocks));
+    if (wide) agb::dz_kernel<8><<<grid, agb::kDzThreads, 0, stream>>>(p);
+    else agb::dz_kernel<1><<<grid, agb::kDzThreads, 0, stream>>>(p);
+    if (g->dbias != nullptr)
+      agb::column_sums_kernel<<<static_cast<unsigned>((g->n + 31) / 32), 256, 0, stream>>>(p.partial, blocks, g->n, g->dbias, g->bias_dtype);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+  }
+  if (g->dx != nullptr) {      // dx[m, k] = sum_n dz[m, n] W[n, k]
+    agb::DenseParams p = plain_output(g, g->dx, g->k, g->dtype);
+    if (p.status == nullptr) return agb_fail(AG_E_CUDA, "no status word");
+    if (int rc = run_product({dz, ld, g->m, false, "dz"}, {g->weight, g->ldw, g->k, true, "weight"}, g->n, g->dtype, p, stream)) return rc;
+  }
+  if (g->dweight != nullptr) {      // dW[n, k] = sum_m dz[m, n] x[m, k]
+    agb::DenseParams p = plain_output(g, g->dweight, g->k, g->dtype);
+    if (p.status == nullptr) return agb_fail(AG_E_CUDA, "no status word");
+    if (int rc = run_product({dz, ld, g->n, true, "dz"}, {g->x, g->ldx, g->k, true, "x"}, g->m, g->dtype, p, stream)) return rc;
+  }
+  return AG_OK;
+}
+
+}  // extern "C"

@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(256) quant_rows_wide_kernel(const __nv_bfloat1
 }
 
 // dst[dst_rows ? dst_rows[i] : i] = src[src_rows ? src_rows[i] : i] for i < rows; one warp per row, 16-byte vectors.
+// No destination (negative) writes nothing, no source writes zeros: the entries of pairs and rows that routing left out.
 __global__ void __launch_bounds__(256) move_rows_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst,
                                                         const long long* __restrict__ src_rows, const long long* __restrict__ dst_rows,
                                                         long long rows, int vec_per_row) {
@@ -166,12 +167,14 @@ __global__ void __launch_bounds__(256) move_rows_kernel(const uint4* __restrict_
   if (w >= rows) return;
   const long long s = src_rows ? src_rows[w] : w;
   const long long d = dst_rows ? dst_rows[w] : w;
+  if (d < 0) return;
   const uint4* sp = src + s * vec_per_row;
   uint4* dp = dst + d * vec_per_row;
-  for (int i = lane; i < vec_per_row; i += 32) dp[i] = sp[i];
+  for (int i = lane; i < vec_per_row; i += 32) dp[i] = s < 0 ? make_uint4(0, 0, 0, 0) : sp[i];
 }
 
-// y[t] = sum_j w[t, j] * rows[pos[t * k + j]] in fp32, rounded once to bf16. One CTA per token, 8 columns per thread.
+// y[t] = sum_j w[t, j] * rows[pos[t * k + j]] in fp32, rounded once to bf16; slots without a row (negative pos) add nothing.
+// One CTA per token, 8 columns per thread.
 __global__ void __launch_bounds__(256) combine_topk_kernel(const __nv_bfloat16* __restrict__ rows, const long long* __restrict__ pos,
                                                            const float* __restrict__ w, __nv_bfloat16* __restrict__ y, int top_k, int cols) {
   const long long t = blockIdx.x;
@@ -179,6 +182,7 @@ __global__ void __launch_bounds__(256) combine_topk_kernel(const __nv_bfloat16* 
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < top_k; ++j) {
       const long long r = pos != nullptr ? pos[t * top_k + j] : t * top_k + j;
+      if (r < 0) continue;
       const float wt = w[t * top_k + j];
       const uint4 v = *reinterpret_cast<const uint4*>(rows + r * cols + c);
       const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
@@ -233,6 +237,7 @@ __global__ void __launch_bounds__(256) combine_topk_f32_kernel(const float* __re
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < top_k; ++j) {
       const long long r = pos[t * top_k + j];
+      if (r < 0) continue;
       const float wt = w[t * top_k + j];
       const float4 v = *reinterpret_cast<const float4*>(rows + r * cols + c);
       acc[0] = fmaf(wt, v.x, acc[0]); acc[1] = fmaf(wt, v.y, acc[1]); acc[2] = fmaf(wt, v.z, acc[2]); acc[3] = fmaf(wt, v.w, acc[3]);
@@ -245,9 +250,142 @@ __global__ void __launch_bounds__(256) combine_topk_f32_kernel(const float* __re
   }
 }
 
+// Gradient of the combine. One CTA per token: its dy row is read once, each of its result rows once, and each gradient row
+// is written once; nothing else moves, so the kernel is bound by memory. A thread holds 8 columns of dy and walks the slots in
+// chunks of 8, whose loads are independent of each other (8 x 16 bytes in flight per thread).
+//   dweights[t, j] = <dy[t], rows[pos]> (fp32, threads' parts joined in a fixed order), drows[pos] = w[t, j] * dy[t].
+constexpr int kGradThreads = 128;
+
+__device__ __forceinline__ void unpack8(const __nv_bfloat16* src, float (&v)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(src);
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __low2float(p[i]);
+    v[2 * i + 1] = __high2float(p[i]);
+  }
+}
+__device__ __forceinline__ void unpack8(const float* src, float (&v)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* dst, const float (&v)[8]) {
+  uint4 u;
+  __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(dst) = u;
+}
+__device__ __forceinline__ void store8(float* dst, const float (&v)[8]) {
+  reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const __nv_bfloat16* __restrict__ dy, const T* __restrict__ rows, long long num_rows,
+                                                                    const long long* __restrict__ pos, const float* __restrict__ w, int top_k, int cols,
+                                                                    T* __restrict__ drows, float* __restrict__ dweights,
+                                                                    unsigned char* __restrict__ row_seen, int* __restrict__ status) {
+  constexpr int J = 8;
+  __shared__ float part[kGradThreads / 32][J];
+  const long long t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int j0 = 0; j0 < top_k; j0 += J) {
+    long long row[J];
+    float wt[J], acc[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      row[j] = -1;
+      wt[j] = acc[j] = 0.f;
+      if (j0 + j < top_k) {
+        const long long pair = t * top_k + j0 + j;
+        const long long r = pos != nullptr ? pos[pair] : pair;
+        if (r >= 0 && r < num_rows) row[j] = r;
+        wt[j] = w[pair];
+      }
+    }
+    if (drows != nullptr && threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < top_k) {
+      const long long pair = t * top_k + j0 + threadIdx.x;
+      const long long r = pos != nullptr ? pos[pair] : pair;
+      if (r >= 0 && r < num_rows) {
+        // one byte of the word that holds it, so that a second pair with the same row finds it set
+        unsigned* word = reinterpret_cast<unsigned*>(row_seen) + (r >> 2);
+        const unsigned bit = 1u << (8 * (r & 3));
+        if ((atomicOr(word, bit) & bit) != 0 && status != nullptr) atomicCAS(status, 0, AG_COMBINE_ROW_TWICE);
+      }
+    }
+    for (int c = threadIdx.x * 8; c < cols; c += kGradThreads * 8) {
+      float g[8];
+      unpack8(dy + t * cols + c, g);
+      if (dweights != nullptr) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (row[j] < 0) continue;
+          float v[8];
+          unpack8(rows + row[j] * cols + c, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[j] = fmaf(g[i], v[i], acc[j]);
+        }
+      }
+      if (drows != nullptr) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (row[j] < 0) continue;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = wt[j] * g[i];
+          store8(drows + row[j] * cols + c, v);
+        }
+      }
+    }
+    if (dweights != nullptr) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+        if (lane == 0) part[warp][j] = acc[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < top_k) {
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < kGradThreads / 32; ++v) sum += part[v][threadIdx.x];
+        dweights[t * top_k + j0 + threadIdx.x] = sum;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Rows that no pair named (padding of the layout) have gradient 0. One warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) zero_unseen_rows_kernel(T* __restrict__ drows, const unsigned char* __restrict__ row_seen, long long num_rows,
+                                                               int cols) {
+  const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  if (r >= num_rows || row_seen[r] != 0) return;
+  const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int c = (threadIdx.x & 31) * 8; c < cols; c += 256) store8(drows + r * cols + c, zero);
+}
+
 }  // namespace agb
 
 namespace {
+template <typename T>
+cudaError_t launch_combine_grad(const void* dy, const void* rows, long long num_rows, const long long* pos, const float* w, long long tokens, int top_k,
+                                int cols, void* drows, float* dweights, void* row_seen, int* status, cudaStream_t stream) {
+  if (drows != nullptr && num_rows > 0) {
+    cudaError_t e = cudaMemsetAsync(row_seen, 0, static_cast<size_t>((num_rows + 3) / 4 * 4), stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (tokens > 0)
+    agb::combine_grad_kernel<T><<<static_cast<unsigned>(tokens), agb::kGradThreads, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(dy), static_cast<const T*>(rows), num_rows, pos, w, top_k, cols, static_cast<T*>(drows), dweights,
+        static_cast<unsigned char*>(row_seen), status);
+  if (drows != nullptr && num_rows > 0)
+    agb::zero_unseen_rows_kernel<T><<<static_cast<unsigned>((num_rows + 7) / 8), 256, 0, stream>>>(
+        static_cast<T*>(drows), static_cast<const unsigned char*>(row_seen), num_rows, cols);
+  return cudaGetLastError();
+}
 int launch_check() {
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
@@ -357,6 +495,28 @@ int ag_combine_topk_f32(const void* rows_f32, const int64_t* pos, const float* w
       static_cast<const float*>(rows_f32), reinterpret_cast<const long long*>(pos), weights, static_cast<__nv_bfloat16*>(y_bf16), top_k,
       static_cast<int>(cols));
   return launch_check();
+}
+
+int ag_combine_topk_backward(const void* dy_bf16, const void* rows, int32_t rows_fp32, int64_t num_rows, const int64_t* pos, const float* weights,
+                             int64_t tokens, int32_t top_k, int64_t cols, void* drows, float* dweights, void* row_seen, int32_t* status,
+                             void* stream) {
+  if (tokens < 0 || top_k <= 0 || num_rows < 0 || cols <= 0 || cols % 8 != 0 || cols > 0x7fffffff || tokens > 0x7fffffff ||
+      num_rows > 8LL * 0x7fffffff)
+    return agb_fail(AG_E_INVALID, "bad sizes (cols must be a multiple of 8)");
+  if (!aligned16(dy_bf16) || !aligned16(rows) || !aligned16(drows) || !aligned_to(pos, 8) || !aligned_to(weights, 4) || !aligned_to(dweights, 4) ||
+      !aligned_to(row_seen, 4))
+    return agb_fail(AG_E_INVALID, "dy, rows and drows must be 16-byte aligned, row_seen 4-byte aligned");
+  if (tokens > 0 && (dy_bf16 == nullptr || weights == nullptr || (dweights != nullptr && rows == nullptr && num_rows > 0)))
+    return agb_fail(AG_E_INVALID, "dy, rows and weights must be non-NULL");
+  if (drows != nullptr && row_seen == nullptr) return agb_fail(AG_E_INVALID, "drows wants row_seen (num_rows bytes, rounded up to a multiple of 4)");
+  if (drows == nullptr && (dweights == nullptr || tokens == 0)) return AG_OK;
+  const long long* at = reinterpret_cast<const long long*>(pos);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e =
+      rows_fp32 ? launch_combine_grad<float>(dy_bf16, rows, num_rows, at, weights, tokens, top_k, static_cast<int>(cols), drows, dweights, row_seen, status, s)
+                : launch_combine_grad<__nv_bfloat16>(dy_bf16, rows, num_rows, at, weights, tokens, top_k, static_cast<int>(cols), drows, dweights, row_seen,
+                                                     status, s);
+  return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
 }
 
 }  // extern "C"

@@ -1,0 +1,790 @@
+// Routing of tokens to experts: scores, group-limited top-k and weights from router logits, the gradient of the weights
+// with respect to the logits, and the tables of the grouped GEMM's layouts that follow from the routing.
+//
+// Callers of the reference do these steps with torch softmax / topk / sort / bincount
+// (asym_gemm/unified_moe/runtime.py:1422-1476).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <cstdint>
+
+#include "../../include/asymgemm_b200.h"
+
+int agb_fail(int code, const char* message);
+
+namespace agb {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kRouteMaxTopK = 32;       // one lane of the token's warp per chosen expert
+constexpr int kRouteMaxPerLane = 32;    // experts held by one lane
+constexpr int kLayoutMaxExperts = 1024;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float warp_max_f(float v) {
+  float r;   // sm_100a reduces floats across the warp in one instruction
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_sum_f(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_max_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// A logit as the router counts it: NaN and -inf switch the expert off, +inf is the largest finite number.
+__device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
+
+struct RouteParams {
+  const void* logits;
+  const float* bias;
+  const int* rows_used;
+  long long* ids;
+  float* weights;
+  long long tokens, ld;
+  int experts, top_k, groups, top_groups, group_size, lanes_per_group, per_lane;
+  int sigmoid, group_max, renormalize, vector_rows;
+  float scale;
+};
+
+// ------------------------------------------------------------------------------------------------ forward
+// One warp per token. The experts of a group lie on `lanes_per_group` (a power of two) neighbouring lanes, `per_lane`
+// consecutive ones each, so the lane order is the expert order, a group's two best scores are a short shuffle
+// reduction, and "lowest index among equals" is "lowest lane, then lowest slot". The k best are taken one at a time: a
+// warp-wide maximum of the lanes' own maxima (one redux), the first lane that holds it gives its expert up.
+//
+// Order. With neither bias nor groups the experts are ordered by their logits, which are exact. Otherwise two experts
+// (or two groups) whose fp32 scores are closer than fp32 resolves could come out in either order; `tol` bounds what the
+// fp32 scores are off by, and a token with two neighbours inside it -- one in a thousand -- is decided once more in 64 bits
+// (route_exact), so that the result is that of the formulas whatever the last bits of expf are.
+struct Slots {
+  int first, count;      // this lane holds the experts first .. first + count - 1
+  __device__ __forceinline__ Slots(const RouteParams& p, int lane) {
+    const int g = lane / p.lanes_per_group, in = (lane % p.lanes_per_group) * p.per_lane;
+    first = g * p.group_size + in;
+    count = g < p.groups ? max(0, min(p.per_lane, p.group_size - in)) : 0;
+  }
+};
+
+// The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left).
+template <typename T, int VPL>
+__device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
+  const Slots at(p, lane);
+  double c[VPL];
+  double mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    c[j] = j < at.count ? static_cast<double>(clean(to_float(row[at.first + j]))) : -INFINITY;
+    mx = fmax(mx, c[j]);
+  }
+  mx = warp_max_d(mx);
+  double sum = 0;
+  if (!p.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? exp(c[j] - mx) : 0;
+    sum = warp_sum_d(sum);
+  }
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    if (c[j] == -INFINITY) continue;
+    c[j] = p.sigmoid ? 1 / (1 + exp(-c[j])) : exp(c[j] - mx) / sum;
+    if (p.bias != nullptr) {
+      const float b = clean(p.bias[at.first + j]);
+      c[j] = b == -INFINITY ? -INFINITY : c[j] + static_cast<double>(b);
+    }
+  }
+  if (p.groups > 1) {
+    double a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      a2 = fmax(a2, fmin(a1, c[j]));
+      a1 = fmax(a1, c[j]);
+    }
+    for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+      const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+      a2 = fmax(fmax(a2, b2), fmin(a1, b1));
+      a1 = fmax(a1, b1);
+    }
+    const double mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
+    const int g = lane / p.lanes_per_group;
+    int rank = 0;
+    for (int o = 0; o < p.groups; ++o) {
+      const double other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
+      rank += other > mine || (other == mine && o < g);
+    }
+    if (rank >= p.top_groups) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) c[j] = -INFINITY;
+    }
+  }
+  // without a bias the scores rise with the logits: among the groups kept, the logits themselves are the exact order
+  if (p.bias == nullptr) {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (c[j] > -INFINITY) c[j] = static_cast<double>(clean(to_float(row[at.first + j])));
+  }
+  int chosen = -1;
+  for (int i = 0; i < p.top_k; ++i) {
+    double m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) m = fmax(m, c[j]);
+    const double best = warp_max_d(m);
+    if (best == -INFINITY) break;
+    const int w = __ffs(__ballot_sync(kAll, m == best)) - 1;
+    int e = -1;
+    if (lane == w) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+        if (e < 0 && c[j] == best) {
+          e = at.first + j;
+          c[j] = -INFINITY;
+        }
+    }
+    e = __shfl_sync(kAll, e, w);
+    if (lane == i) chosen = e;
+  }
+  return chosen;
+}
+
+// Slots of one lane from memory. `vector_rows`: every lane's slots are full and 16-byte aligned.
+template <typename T, int VPL>
+__device__ __forceinline__ void load_slots(const RouteParams& p, const T* row, const Slots& at, float (&l)[VPL]) {
+  constexpr int kBytes = VPL * static_cast<int>(sizeof(T));
+  if constexpr (kBytes >= 16) {
+    if (p.vector_rows) {
+#pragma unroll
+      for (int q = 0; q < kBytes / 16; ++q) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (at.count > 0) v = __ldg(reinterpret_cast<const uint4*>(row + at.first) + q);
+        const T* t = reinterpret_cast<const T*>(&v);
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) l[q * kPer + i] = at.count > 0 ? clean(to_float(t[i])) : -INFINITY;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) l[j] = j < at.count ? clean(to_float(row[at.first + j])) : -INFINITY;
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
+  const long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (token >= p.tokens) return;
+  long long* ids = p.ids + token * p.top_k;
+  float* weights = p.weights + token * p.top_k;
+  if (p.rows_used != nullptr && token >= *p.rows_used) {      // a padding token is routed nowhere
+    if (lane < p.top_k) {
+      ids[lane] = -1;
+      weights[lane] = 0.f;
+    }
+    return;
+  }
+  const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+  const bool scored = p.bias != nullptr || p.groups > 1;      // the order needs the scores, not just the logits
+
+  const Slots at(p, lane);
+  float c[VPL];      // what the experts are ordered by; -inf = off or taken
+  load_slots<T, VPL>(p, row, at, c);
+  float mx = c[0];
+#pragma unroll
+  for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
+  float row_max = 0.f, sum = 0.f;
+  if (!p.sigmoid && (scored || !p.renormalize)) {
+    row_max = warp_max_f(mx);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? expf(c[j] - row_max) : 0.f;
+    sum = warp_sum_f(sum);
+  }
+  bool unsure = false;
+  float tol = 0.f;
+  if (scored) {
+    float s[VPL];
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      if (p.sigmoid) s[j] = 1.f / (1.f + expf(-c[j]));
+      else s[j] = expf(c[j] - row_max) * inv;
+      if (c[j] == -INFINITY) s[j] = -INFINITY;
+    }
+    // Error of a score: sigmoid, below 8 roundings of a number <= 1; softmax, of numbers <= 1 / sum: the argument's
+    // rounding, d e^-d 2^-24 at most for l = max - d, and up to 37 additions in the sum. A bias adds half a step of the result.
+    tol = p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const float b = j < at.count ? clean(__ldg(p.bias + at.first + j)) : -INFINITY;
+        s[j] = s[j] == -INFINITY || b == -INFINITY ? -INFINITY : s[j] + b;
+      }
+    }
+    if (p.groups > 1) {
+      float a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        a2 = fmaxf(a2, fminf(a1, s[j]));
+        a1 = fmaxf(a1, s[j]);
+      }
+      for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+        const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+        a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
+        a1 = fmaxf(a1, b1);
+      }
+      const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
+      const int g = lane / p.lanes_per_group;
+      int rank = 0;
+      for (int o = 0; o < p.groups; ++o) {
+        const float other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
+        rank += other > mine || (other == mine && o < g);
+      }
+      const bool kept = rank < p.top_groups;
+      const bool real = g < p.groups;
+      // the weakest group kept against the strongest one left out
+      const float low = -warp_max_f(real && kept ? -mine : -INFINITY), high = warp_max_f(real && !kept ? mine : -INFINITY);
+      if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
+      if (!kept) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) s[j] = c[j] = -INFINITY;
+      }
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) c[j] = s[j];
+    }
+    mx = c[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
+  }
+
+  int chosen = -1;
+  float last = 0.f;
+  int last_e = 0;
+  const int rounds = p.bias != nullptr ? p.top_k + 1 : p.top_k;    // one more, to see how far the first one left out is
+  for (int i = 0; i < rounds && !unsure; ++i) {
+    const float best = warp_max_f(mx);
+    if (best == -INFINITY) break;
+    const int w = __ffs(__ballot_sync(kAll, mx == best)) - 1;
+    int e = -1;
+    if (lane == w) {
+      mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        if (e < 0 && c[j] == best) {
+          e = at.first + j;
+          c[j] = -INFINITY;
+        }
+        mx = fmaxf(mx, c[j]);
+      }
+    }
+    e = __shfl_sync(kAll, e, w);
+    if (p.bias != nullptr) {
+      if (i > 0 && !(last - best > 2.f * tol + 0x1p-21f * (fabsf(last) + fabsf(best))))
+        // equal logits with equal biases are equal whatever the arithmetic: lowest index first, as taken here
+        unsure = last != best || clean(to_float(row[e])) != clean(to_float(row[last_e])) || clean(p.bias[e]) != clean(p.bias[last_e]);
+      last = best;
+      last_e = e;
+    }
+    if (lane == i) chosen = e;
+  }
+  if (lane >= p.top_k) chosen = -1;
+  if (unsure) chosen = route_exact<T, VPL>(p, row, lane);
+
+  // Weights, lane i for the expert chosen i-th. Sums over at most 32 chosen experts, in fp32.
+  const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
+  float w = 0.f;
+  if (p.renormalize) {
+    // scores up to a common factor: shifting by the largest chosen logit (sigmoid: only where all are negative) keeps
+    // rows of very small scores away from 0 / 0
+    float top = warp_max_f(l);
+    if (p.sigmoid) {
+      top = fminf(top, 0.f);
+      w = l >= 0.f ? 1.f / (1.f + expf(-l)) : expf(l - top) / (1.f + expf(l));
+    } else {
+      w = expf(l - top);
+    }
+    if (chosen < 0) w = 0.f;
+    const float total = warp_sum_f(w);
+    w = chosen >= 0 ? w / total : 0.f;
+  } else if (chosen >= 0) {
+    w = p.sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - row_max) / sum;
+  }
+  if (lane < p.top_k) {
+    ids[lane] = chosen;
+    weights[lane] = w * p.scale;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// dlogits of one token per warp. Weights w_i = scale * s_i (/ S, S = sum of the chosen scores), gradients g_i:
+//   renormalised:  dl_i = scale * q_i * d_i * (g_i - sum_j q_j g_j),  q = s / S,  d = 1 (softmax) or 1 - s_i (sigmoid);
+//   sigmoid:       dl_i = scale * g_i * s_i * (1 - s_i);
+//   softmax:       dl_j = scale * s_j * ([j chosen] g_j - sum_i s_i g_i), for every expert j.
+// Experts that do not appear get 0, so only the last form reads the whole row; all write it, once, in 16-byte pieces.
+struct RouteGradParams {
+  const void* logits;
+  const float* dweights;
+  const long long* ids;
+  void* dlogits;
+  long long tokens, ld;
+  int experts, top_k, sigmoid, renormalize, vector_rows;
+  float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGradParams p) {
+  const long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (token >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+  T* out = static_cast<T*>(p.dlogits) + token * p.experts;
+  const bool dense = !p.sigmoid && !p.renormalize;
+  int id = -1;
+  float g = 0.f;
+  if (lane < p.top_k) {
+    const long long e = p.ids[token * p.top_k + lane];
+    if (e >= 0 && e < p.experts) {
+      id = static_cast<int>(e);
+      g = p.dweights[token * p.top_k + lane] * p.scale;
+    }
+  }
+  const float l = id >= 0 ? clean(to_float(row[id])) : -INFINITY;
+  if (l == -INFINITY) id = -1;
+  float v = 0.f, row_max = 0.f, inv = 0.f, dot = 0.f;
+  if (p.renormalize) {
+    float top = warp_max_f(l), s = 0.f, rest = 1.f;
+    if (p.sigmoid) {
+      top = fminf(top, 0.f);
+      const float t = expf(-fabsf(l));
+      rest = (l >= 0.f ? t : 1.f) / (1.f + t);                       // 1 - sigmoid(l), without cancellation
+      s = l >= 0.f ? 1.f / (1.f + t) : expf(l - top) / (1.f + t);
+    } else {
+      s = expf(l - top);
+    }
+    if (id < 0) s = 0.f;
+    const float total = warp_sum_f(s);
+    const float q = id >= 0 ? s / total : 0.f;
+    v = q * rest * (g - warp_sum_f(q * g));
+  } else if (p.sigmoid) {
+    const float t = expf(-fabsf(l));
+    v = id >= 0 ? g * t / ((1.f + t) * (1.f + t)) : 0.f;             // s (1 - s)
+  } else {
+    float mx = -INFINITY;
+    for (int e = lane; e < p.experts; e += 32) mx = fmaxf(mx, clean(to_float(row[e])));
+    row_max = warp_max_f(mx);
+    float sum = 0.f;
+    for (int e = lane; e < p.experts; e += 32) {
+      const float x = clean(to_float(row[e]));
+      sum += x > -INFINITY ? expf(x - row_max) : 0.f;
+    }
+    sum = warp_sum_f(sum);
+    inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float s = id >= 0 ? expf(l - row_max) * inv : 0.f;
+    dot = warp_sum_f(s * g);
+    v = s * g;
+  }
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  const int step = p.vector_rows ? V : 1;
+  for (int e0 = lane * step; e0 - lane * step < p.experts; e0 += 32 * step) {   // every lane of the warp takes every round
+    float a[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      a[i] = 0.f;
+      if (dense && i < step && e0 + i < p.experts) {
+        const float x = clean(to_float(row[e0 + i]));
+        if (x > -INFINITY) a[i] = -expf(x - row_max) * inv * dot;
+      }
+    }
+    for (int t = 0; t < p.top_k; ++t) {      // an expert named twice in a row gets both parts
+      const int at = __shfl_sync(kAll, id, t) - e0;
+      const float add = __shfl_sync(kAll, v, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (at == i) a[i] += add;
+    }
+    if (p.vector_rows) {
+      if (e0 < p.experts) {
+        uint4 o;
+        T* t = reinterpret_cast<T*>(&o);
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = from_float<T>(a[i]);
+        *reinterpret_cast<uint4*>(out + e0) = o;
+      }
+    } else if (e0 < p.experts) {
+      out[e0] = from_float<T>(a[0]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ layout tables
+// A stable counting sort of the (token, slot) pairs by expert, on integers only: the same input gives the same tables.
+// Every block owns a run of consecutive pairs, every warp of it a run of those. How many pairs of an expert lie before
+// a warp's run follows from the blocks' counts (first kernel, or the one block's own) and the warps' counts (shared
+// memory); inside a warp 32 pairs are ranked at a time with match.any.
+struct LayoutParams {
+  const void* ids;
+  int ids_64;
+  long long pairs;
+  int top_k, experts, alignment, max_rows;    // max_rows > 0: the masked layout
+  long long rows;                             // rows of the layout = entries of row_token
+  int* block_counts;                          // [blocks, experts]
+  long long* pair_row;
+  long long* row_token;
+  long long* rows_per_expert;                 // contiguous
+  int* offsets;                               // contiguous [2 * experts]
+  int* expert_list;                           // contiguous [experts + 1]
+  int* masked_m;                              // masked [experts]
+  int* status;
+  long long run;                              // pairs per block, a multiple of the block's threads
+};
+
+constexpr int kLayoutThreads = 1024;
+constexpr int kLayoutWarps = kLayoutThreads / 32;
+
+__device__ __forceinline__ int pair_expert(const LayoutParams& p, long long i, bool report) {
+  const long long e = p.ids_64 ? __ldg(static_cast<const long long*>(p.ids) + i) : __ldg(static_cast<const int*>(p.ids) + i);
+  if (e >= 0 && e < p.experts) return static_cast<int>(e);
+  if (report && e != -1 && p.status != nullptr) atomicCAS(p.status, 0, AG_EP_BAD_EXPERT | (static_cast<int>(blockIdx.x) << 8));
+  return -1;
+}
+
+__global__ void __launch_bounds__(kLayoutThreads) layout_count_kernel(const LayoutParams p) {
+  extern __shared__ int count[];
+  for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) count[e] = 0;
+  __syncthreads();
+  const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
+  for (long long i = begin + threadIdx.x; i < end; i += kLayoutThreads) {
+    const int e = pair_expert(p, i, false);
+    if (e >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) p.block_counts[static_cast<long long>(blockIdx.x) * p.experts + e] = count[e];
+}
+
+// ONE: the launch is a single block, which needs no counts of others.
+template <bool ONE>
+__global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const LayoutParams p) {
+  extern __shared__ int smem[];
+  int* total = smem;                    // [experts] pairs of the expert
+  int* start = total + p.experts;       // [experts + 1] first row of its segment
+  int* seen = start + p.experts + 1;    // [experts] its pairs in the blocks before this one
+  int* mine = seen + p.experts;         // [warps, experts] its pairs in each warp's run, then those before the run
+  __shared__ int warp_sums[kLayoutWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int E = p.experts;
+  for (int e = threadIdx.x; e < E; e += kLayoutThreads) total[e] = seen[e] = 0;
+  for (int i = threadIdx.x; i < kLayoutWarps * E; i += kLayoutThreads) mine[i] = 0;
+  __syncthreads();
+
+  const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
+  const long long share = p.run / kLayoutWarps;            // a multiple of 32
+  const long long from = begin + warp * share, to = min(from + share, end);
+  for (long long i0 = from; i0 < to; i0 += 32) {
+    const int e = i0 + lane < to ? pair_expert(p, i0 + lane, true) : -1;
+    const unsigned same = __match_any_sync(kAll, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] += __popc(same);
+    __syncwarp();
+  }
+  if (!ONE) {
+    // all blocks' counts, `parts` threads per expert; integer sums, so their order does not matter
+    const int parts = max(1, kLayoutThreads / E);
+    for (int i = threadIdx.x; i < parts * E; i += kLayoutThreads) {
+      const int e = i % E;
+      int all = 0, before = 0;
+      for (int b = i / E; b < static_cast<int>(gridDim.x); b += parts) {
+        const int v = __ldg(p.block_counts + static_cast<long long>(b) * E + e);
+        all += v;
+        before += b < static_cast<int>(blockIdx.x) ? v : 0;
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&seen[e], before);
+    }
+  }
+  __syncthreads();
+  // pairs of the expert before each warp's run, in this block
+  for (int e = threadIdx.x; e < E; e += kLayoutThreads) {
+    int before = seen[e];
+    for (int w = 0; w < kLayoutWarps; ++w) {
+      const int v = mine[w * E + e];
+      mine[w * E + e] = before;
+      before += v;
+    }
+    if (ONE) total[e] = before;
+  }
+  __syncthreads();
+  // first row of every segment: a running sum over the experts, one per thread
+  {
+    const int e = threadIdx.x;
+    int size = 0;
+    if (e < E) size = p.max_rows > 0 ? p.max_rows : (total[e] + p.alignment - 1) / p.alignment * p.alignment;
+    int sum = size;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kAll, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      int v = warp_sums[lane], s = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kAll, s, o);
+        if (lane >= o) s += u;
+      }
+      warp_sums[lane] = s - v;
+    }
+    __syncthreads();
+    sum += warp_sums[warp];
+    if (e < E) {
+      start[e] = sum - size;
+      if (e == E - 1) start[E] = sum;
+      if (blockIdx.x == 0) {
+        if (p.max_rows > 0) {
+          p.masked_m[e] = min(total[e], p.max_rows);
+        } else {
+          p.rows_per_expert[e] = total[e];
+          p.offsets[2 * e] = sum - size;
+          p.offsets[2 * e + 1] = sum;
+          p.expert_list[e] = e;
+          if (e == E - 1) p.expert_list[E] = -1;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (long long i0 = from; i0 < to; i0 += 32) {
+    const long long i = i0 + lane;
+    const int e = i < to ? pair_expert(p, i, false) : -1;
+    const unsigned same = __match_any_sync(kAll, e);
+    int base = 0;
+    if (e >= 0) base = mine[warp * E + e];
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] = base + __popc(same);
+    __syncwarp();
+    if (i < to) {
+      const int within = base + __popc(same & ((1u << lane) - 1u));
+      const bool placed = e >= 0 && (p.max_rows == 0 || within < p.max_rows);
+      const long long row = placed ? static_cast<long long>(start[e]) + within : -1;
+      p.pair_row[i] = row;
+      if (placed) p.row_token[row] = i / p.top_k;
+    }
+  }
+  // rows that no pair has: -1, each block a run of them
+  const long long rows_run = (p.rows + gridDim.x - 1) / gridDim.x;
+  const long long r_end = min((blockIdx.x + 1) * rows_run, p.rows);
+  for (long long r = blockIdx.x * rows_run + threadIdx.x; r < r_end; r += kLayoutThreads) {
+    if (r >= start[E]) {
+      p.row_token[r] = -1;
+      continue;
+    }
+    int lo = 0, hi = E;                // the last segment that starts at or before r (empty ones share their start with the next)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= r) lo = mid;
+      else hi = mid;
+    }
+    if (r - start[lo] >= total[lo]) p.row_token[r] = -1;
+  }
+}
+
+}  // namespace agb
+
+namespace {
+
+int launch_check() {
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+}
+bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+int size_of(int dtype) { return dtype == AG_T_FP32 ? 4 : 2; }
+
+template <typename T>
+void launch_route(const agb::RouteParams& p, cudaStream_t stream) {
+  constexpr int kWarps = 4;
+  const unsigned grid = static_cast<unsigned>((p.tokens + kWarps - 1) / kWarps);
+  if (p.per_lane <= 1) agb::route_topk_kernel<T, 1><<<grid, 32 * kWarps, 0, stream>>>(p);
+  else if (p.per_lane <= 2) agb::route_topk_kernel<T, 2><<<grid, 32 * kWarps, 0, stream>>>(p);
+  else if (p.per_lane <= 4) agb::route_topk_kernel<T, 4><<<grid, 32 * kWarps, 0, stream>>>(p);
+  else if (p.per_lane <= 8) agb::route_topk_kernel<T, 8><<<grid, 32 * kWarps, 0, stream>>>(p);
+  else if (p.per_lane <= 16) agb::route_topk_kernel<T, 16><<<grid, 32 * kWarps, 0, stream>>>(p);
+  else agb::route_topk_kernel<T, 32><<<grid, 32 * kWarps, 0, stream>>>(p);
+}
+
+// Pairs per block: 4096 keep one block for a decode batch, and no more than 128 blocks, because every block sums the
+// counts of all others.
+long long layout_run(long long pairs) {
+  const long long run = (pairs + 127) / 128;
+  const long long least = run > 4096 ? run : 4096;
+  return (least + agb::kLayoutThreads - 1) / agb::kLayoutThreads * agb::kLayoutThreads;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ag_route_topk(const ag_route_desc_t* r) {
+  if (r == nullptr) return agb_fail(AG_E_INVALID, "desc is NULL");
+  if (r->dtype < AG_T_BF16 || r->dtype > AG_T_FP32) return agb_fail(AG_E_INVALID, "logits must be bf16, fp16 or fp32");
+  if (r->tokens < 0 || r->experts <= 0 || r->top_k <= 0 || r->ld < r->experts) return agb_fail(AG_E_INVALID, "bad sizes");
+  if (r->scoring != AG_SCORE_SOFTMAX && r->scoring != AG_SCORE_SIGMOID) return agb_fail(AG_E_INVALID, "unknown scoring");
+  if (r->groups <= 0 || r->groups > 32 || r->experts % r->groups != 0 || r->top_groups <= 0 || r->top_groups > r->groups)
+    return agb_fail(AG_E_INVALID, "the groups (1 .. 32) must divide the experts, and top_groups must be 1 .. groups");
+  const int size = r->experts / r->groups;
+  if (r->top_k > agb::kRouteMaxTopK || r->top_k > r->top_groups * size)
+    return agb_fail(AG_E_INVALID, "top_k must be at most 32 and at most the experts of top_groups groups");
+  int lanes = 32;
+  while (lanes * r->groups > 32) lanes >>= 1;
+  const int per = (size + lanes - 1) / lanes;
+  if (per > agb::kRouteMaxPerLane) return agb_fail(AG_E_INVALID, "too many experts (at most 32 per lane: 1024 in one group, 1024 / groups rounded to a power of two in each of several)");
+  if (!aligned_to(r->logits, size_of(r->dtype)) || !aligned_to(r->bias, 4) || !aligned_to(r->rows_used, 4) || !aligned_to(r->ids, 8) ||
+      !aligned_to(r->weights, 4))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  if (r->tokens == 0) return AG_OK;
+  if (r->logits == nullptr || r->ids == nullptr || r->weights == nullptr) return agb_fail(AG_E_INVALID, "logits, ids and weights must be non-NULL");
+  if (r->tokens > 4LL * 0x7fffffff) return agb_fail(AG_E_INVALID, "too many tokens");
+  agb::RouteParams p{};
+  p.logits = r->logits;
+  p.bias = r->bias;
+  p.rows_used = r->rows_used;
+  p.ids = reinterpret_cast<long long*>(r->ids);
+  p.weights = r->weights;
+  p.tokens = r->tokens;
+  p.ld = r->ld;
+  p.experts = r->experts;
+  p.top_k = r->top_k;
+  p.groups = r->groups;
+  p.top_groups = r->top_groups;
+  p.group_size = size;
+  p.lanes_per_group = lanes;
+  // a power of two of slots where that fills the lanes exactly (vector loads), else as few as hold the group
+  p.per_lane = per;
+  p.sigmoid = r->scoring == AG_SCORE_SIGMOID;
+  p.group_max = r->group_max != 0;
+  p.renormalize = r->renormalize != 0;
+  p.scale = r->scale;
+  const bool pow2 = (per & (per - 1)) == 0;
+  p.vector_rows = pow2 && size == per * lanes && per * size_of(r->dtype) >= 16 && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
+  cudaStream_t stream = static_cast<cudaStream_t>(r->stream);
+  if (r->dtype == AG_T_BF16) launch_route<__nv_bfloat16>(p, stream);
+  else if (r->dtype == AG_T_FP16) launch_route<__half>(p, stream);
+  else launch_route<float>(p, stream);
+  return launch_check();
+}
+
+int ag_route_topk_backward(const void* logits, int32_t dtype, int64_t tokens, int64_t ld, int32_t experts, const float* dweights, const int64_t* ids,
+                           int32_t top_k, int32_t scoring, int32_t renormalize, float scale, void* dlogits, void* stream) {
+  if (dtype < AG_T_BF16 || dtype > AG_T_FP32) return agb_fail(AG_E_INVALID, "logits must be bf16, fp16 or fp32");
+  if (tokens < 0 || experts <= 0 || top_k <= 0 || top_k > agb::kRouteMaxTopK || ld < experts || tokens > 4LL * 0x7fffffff)
+    return agb_fail(AG_E_INVALID, "bad sizes (top_k must be 1 .. 32)");
+  if (scoring != AG_SCORE_SOFTMAX && scoring != AG_SCORE_SIGMOID) return agb_fail(AG_E_INVALID, "unknown scoring");
+  const int size = size_of(dtype);
+  if (!aligned_to(logits, size) || !aligned_to(dlogits, size) || !aligned_to(dweights, 4) || !aligned_to(ids, 8))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  if (tokens == 0) return AG_OK;
+  if (!logits || !dweights || !ids || !dlogits) return agb_fail(AG_E_INVALID, "logits, dweights, ids and dlogits must be non-NULL");
+  agb::RouteGradParams p{};
+  p.logits = logits;
+  p.dweights = dweights;
+  p.ids = reinterpret_cast<const long long*>(ids);
+  p.dlogits = dlogits;
+  p.tokens = tokens;
+  p.ld = ld;
+  p.experts = experts;
+  p.top_k = top_k;
+  p.sigmoid = scoring == AG_SCORE_SIGMOID;
+  p.renormalize = renormalize != 0;
+  p.scale = scale;
+  p.vector_rows = static_cast<int64_t>(experts) * size % 16 == 0 && aligned_to(dlogits, 16);
+  const unsigned grid = static_cast<unsigned>((tokens + 3) / 4);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == AG_T_BF16) agb::route_topk_backward_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
+  else if (dtype == AG_T_FP16) agb::route_topk_backward_kernel<__half><<<grid, 128, 0, s>>>(p);
+  else agb::route_topk_backward_kernel<float><<<grid, 128, 0, s>>>(p);
+  return launch_check();
+}
+
+uint64_t ag_route_layout_workspace_bytes(int64_t pairs, int32_t experts) {
+  if (pairs <= 0 || experts <= 0) return 0;
+  const int64_t blocks = (pairs + layout_run(pairs) - 1) / layout_run(pairs);
+  return blocks > 1 ? static_cast<uint64_t>(blocks) * experts * 4 : 0;
+}
+
+int ag_route_layout(const ag_route_layout_desc_t* r) {
+  if (r == nullptr) return agb_fail(AG_E_INVALID, "desc is NULL");
+  if (r->tokens < 0 || r->top_k <= 0 || r->experts <= 0 || r->experts > agb::kLayoutMaxExperts || r->max_rows < 0 || r->rows < 0)
+    return agb_fail(AG_E_INVALID, "bad sizes (at most 1024 experts)");
+  const int64_t pairs = r->tokens * r->top_k;
+  if (pairs > 0x7fffffffLL / 2 || r->rows > 0x7fffffffLL) return agb_fail(AG_E_INVALID, "too many (token, slot) pairs");
+  if (!aligned_to(r->ids, r->ids_64 ? 8 : 4) || !aligned_to(r->pair_row, 8) || !aligned_to(r->row_token, 8) || !aligned_to(r->rows_per_expert, 8) ||
+      !aligned_to(r->offsets, 4) || !aligned_to(r->expert_list, 4) || !aligned_to(r->masked_m, 4) || !aligned_to(r->workspace, 4))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+  if ((pairs > 0 && (r->ids == nullptr || r->pair_row == nullptr)) || (r->rows > 0 && r->row_token == nullptr))
+    return agb_fail(AG_E_INVALID, "ids, pair_row and row_token must be non-NULL");
+  if (r->max_rows > 0) {
+    if (r->masked_m == nullptr || r->rows != static_cast<int64_t>(r->experts) * r->max_rows)
+      return agb_fail(AG_E_INVALID, "the masked layout wants masked_m and experts * max_rows rows");
+  } else {
+    if (r->alignment <= 0 || r->rows_per_expert == nullptr || r->offsets == nullptr || r->expert_list == nullptr)
+      return agb_fail(AG_E_INVALID, "the contiguous layout wants a positive alignment, rows_per_expert, offsets and expert_list");
+    // every expert's segment ends less than one alignment past its pairs
+    if (r->rows < pairs + static_cast<int64_t>(r->experts) * (r->alignment - 1) && r->rows < pairs * r->alignment)
+      return agb_fail(AG_E_INVALID, "rows must cover every expert's padded segment");
+  }
+  const int64_t run = layout_run(pairs);
+  const int blocks = pairs > 0 ? static_cast<int>((pairs + run - 1) / run) : 1;
+  if (blocks > 1 && (r->workspace == nullptr || r->workspace_bytes < ag_route_layout_workspace_bytes(pairs, r->experts)))
+    return agb_fail(AG_E_INVALID, "workspace too small (ag_route_layout_workspace_bytes)");
+  agb::LayoutParams p{};
+  p.ids = r->ids;
+  p.ids_64 = r->ids_64;
+  p.pairs = pairs;
+  p.top_k = r->top_k;
+  p.experts = r->experts;
+  p.alignment = r->alignment;
+  p.max_rows = r->max_rows;
+  p.rows = r->rows;
+  p.block_counts = static_cast<int*>(r->workspace);
+  p.pair_row = reinterpret_cast<long long*>(r->pair_row);
+  p.row_token = reinterpret_cast<long long*>(r->row_token);
+  p.rows_per_expert = reinterpret_cast<long long*>(r->rows_per_expert);
+  p.offsets = r->offsets;
+  p.expert_list = r->expert_list;
+  p.masked_m = r->masked_m;
+  p.status = r->status;
+  p.run = run;
+  cudaStream_t stream = static_cast<cudaStream_t>(r->stream);
+  const size_t smem = (static_cast<size_t>(r->experts) * (3 + agb::kLayoutWarps) + 1) * 4;
+  auto place = blocks == 1 ? agb::layout_place_kernel<true> : agb::layout_place_kernel<false>;
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+  }
+  if (blocks > 1) agb::layout_count_kernel<<<blocks, agb::kLayoutThreads, static_cast<size_t>(r->experts) * 4, stream>>>(p);
+  place<<<blocks, agb::kLayoutThreads, smem, stream>>>(p);
+  return launch_check();
+}
+
+}  // extern "C"

@@ -1,12 +1,16 @@
-"""Python wrappers of the MoE helper kernels (csrc/moe_glue.cu) declared in include/asymgemm_b200.h.
+"""Python wrappers of the MoE helper kernels (csrc/moe_glue.cu, csrc/route.cu) declared in include/asymgemm_b200.h.
 
 CUDA tensors go through the C ABI (and fail loudly if the library is missing). The row-movement helpers also accept
 CPU tensors, where they are plain torch indexing: that branch exists only so that the expert-parallel routing logic can
-be exercised by gloo ranks without a GPU; the quantisers and the GEMMs have no CPU branch.
+be exercised by gloo ranks without a GPU; the quantisers, the router and the GEMMs have no CPU branch.
+
+`route_topk` and `combine_topk` are differentiable: with gradients enabled, calls whose logits, rows or weights require
+one are recorded for autograd. Their gradients are also functions of their own (`route_topk_backward`,
+`combine_topk_backward`), which is the form to capture into a CUDA graph.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -119,8 +123,18 @@ def move_rows_into(out: torch.Tensor, src: torch.Tensor, dst_rows: torch.Tensor)
 
 
 def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
-    """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype; pos None = t*top_k + j."""
+    """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (CUDA: bf16); pos None =
+    t*top_k + j. On CUDA slots with a negative pos (pairs a layout dropped) add nothing, and the call is differentiable with
+    respect to `rows` and `weights`; a row that two slots name has no gradient (see `combine_topk_backward`)."""
+    if rows.is_cuda and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
+    return _combine_topk(rows, pos, weights, tokens, top_k)
+
+
+def _combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
     cols = rows.shape[1]
+    if tokens == 0:
+        return torch.empty((0, cols), dtype=torch.bfloat16 if rows.is_cuda else rows.dtype, device=rows.device)
     if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():
         y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
         w = weights.to(torch.float32).contiguous()
@@ -137,3 +151,126 @@ def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, t
         return y
     picked = (rows.index_select(0, pos) if pos is not None else rows[: tokens * top_k]).view(tokens, top_k, cols).float()
     return (picked * weights.unsqueeze(-1).float()).sum(dim=1).to(rows.dtype)
+
+
+def combine_topk_backward(dy: torch.Tensor, rows: torch.Tensor, pos: Optional[torch.Tensor], weights: torch.Tensor, need_rows: bool = True,
+                          need_weights: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients of `combine_topk` from dy bf16 [tokens, cols]: (drows like rows, dweights fp32 [tokens, top_k]), None for one
+    that is not needed (frozen experts need dweights only, which leaves the rows' half of the memory traffic out).
+
+    dweights[t, j] = <dy[t], rows[pos]> in fp32; drows[pos] = weights[t, j] * dy[t], rounded once, and 0 in rows that no
+    slot names. Slots with a pos outside the rows add nothing. With `need_rows` a row may be named by one slot only, as every
+    layout here does: a second one sets the status word (`check_status` raises). cols must be a multiple of 8."""
+    from . import api
+    w = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.to(torch.float32).contiguous()
+    return _lib.torch_ops().combine_topk_backward(dy, rows, pos, w, bool(need_rows), bool(need_weights), api._status_word(dy.device))
+
+
+class _CombineTopK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, pos, weights, tokens, top_k):
+        ctx.save_for_backward(rows, pos, weights)
+        ctx.top_k = top_k
+        return _combine_topk(rows, pos, weights, tokens, top_k)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        rows, pos, weights = ctx.saved_tensors
+        drows, dweights = combine_topk_backward(dy.contiguous(), rows, pos, weights.reshape(dy.shape[0], ctx.top_k), ctx.needs_input_grad[0],
+                                                ctx.needs_input_grad[2])
+        if dweights is not None:
+            dweights = dweights.view(weights.shape).to(weights.dtype)
+        return drows, None, dweights, None, None
+
+
+# --------------------------------------------------------------------------------------------- routing
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"top2": False, "max": True}
+
+
+def _named(table: dict, name: str, what: str):
+    if name not in table:
+        raise RuntimeError(f"{what} must be one of {', '.join(map(repr, table))}, got {name!r}")
+    return table[name]
+
+
+def route_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+               top_groups: int = 1, group_score: str = "top2", renormalize: bool = True, scale: float = 1.0,
+               rows_used: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Router: logits [tokens, experts] (bf16, fp16 or fp32; rows may be strided) -> (topk_ids int64, topk_weights fp32), both
+    [tokens, top_k], largest first: what `ExpertParallelMoE.forward`, `Int8MoELayer.forward` and `route_layout` take.
+
+    Scores are `softmax` over all experts or `sigmoid`. Experts are chosen by score + `bias` (fp32 [experts], a
+    balance term that does not enter the weights), the lowest index among equals; with `num_groups` > 1 only among the
+    `top_groups` groups of consecutive experts whose two largest (`group_score="top2"`) or largest ("max") such values
+    are best. Weights are the chosen experts' scores, divided by their sum (`renormalize`), times `scale`.
+
+    The order is that of exact arithmetic: fp32 scores too close to tell apart are compared in fp64. A NaN or -inf logit or
+    bias switches an expert off for the token, a +inf logit counts as the largest finite number. Slots for which no expert is
+    left, and all slots of tokens from `rows_used` on (device int32 tensor of one element: a batch padded at its end), get id
+    -1 and weight 0; `route_layout` and `combine_topk` skip them. At most 1024 experts, 32 groups, top_k 32.
+
+    Differentiable with respect to `logits` through the weights (`route_topk_backward`)."""
+    args = (int(top_k), _named(_SCORING, scoring, "scoring"), bias, int(num_groups), int(top_groups),
+            _named(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), float(scale), rows_used)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouteTopK.apply(logits, *args)
+    return _lib.torch_ops().route_topk(logits, *args)
+
+
+def route_topk_backward(dweights: torch.Tensor, topk_ids: torch.Tensor, logits: torch.Tensor, scoring: str = "softmax", renormalize: bool = True,
+                        scale: float = 1.0) -> torch.Tensor:
+    """dlogits [tokens, experts] (type of `logits`) from dweights fp32 [tokens, top_k], the `topk_ids` that `route_topk` chose
+    and its arguments. The choice has no gradient; slots with id -1 add nothing."""
+    return _lib.torch_ops().route_topk_backward(dweights, topk_ids, logits, _named(_SCORING, scoring, "scoring"), bool(renormalize), float(scale))
+
+
+class _RouteTopK(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, *args):
+        ids, weights = _lib.torch_ops().route_topk(logits, *args)
+        ctx.save_for_backward(logits, ids)
+        ctx.how = (args[1], args[6], args[7])
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dweights):
+        logits, ids = ctx.saved_tensors
+        dlogits = _lib.torch_ops().route_topk_backward(dweights.to(torch.float32).contiguous(), ids, logits, *ctx.how)
+        return (dlogits,) + (None,) * 9
+
+
+class RouteLayout(NamedTuple):
+    """Tables of the contiguous layout (`route_layout`)."""
+    pair_row: torch.Tensor         # int64 [tokens * top_k]: row of every (token, slot) pair, -1 = none (`pos` of combine_topk)
+    row_token: torch.Tensor        # int64 [rows]: token of every row, -1 = padding (`src_rows` of move_rows)
+    rows_per_expert: torch.Tensor  # int64 [experts]
+    offsets: torch.Tensor          # int32 [2 * experts]: (start, end) of every expert's padded segment
+    experts: torch.Tensor          # int32 [experts + 1]: 0 .. experts - 1, -1
+
+
+class MaskedRouteLayout(NamedTuple):
+    """Tables of the masked layout (`route_layout_masked`)."""
+    pair_row: torch.Tensor         # int64 [tokens * top_k]: row in the flattened [experts * max_rows], -1 = none or dropped
+    row_token: torch.Tensor        # int64 [experts * max_rows]: token of every row, -1 = unused
+    masked_m: torch.Tensor         # int32 [experts]: rows used
+
+
+def route_layout(topk_ids: torch.Tensor, num_experts: int, alignment: int = 128) -> RouteLayout:
+    """Tables of the contiguous layout of the grouped GEMMs from topk_ids [tokens, top_k] (int64 or int32, CUDA), on the device
+    and without a host synchronisation: pairs sorted by expert, in their own order within one, every expert's segment padded to
+    `alignment` rows. `row_token` has room for the worst case (all pairs plus one alignment per expert), -1 past the last row.
+    Ids of -1 (no expert) get no row; other ids outside [0, num_experts) do neither and set the status word (`check_status`
+    raises). At most 1024 experts."""
+    from . import api
+    return RouteLayout(*_lib.torch_ops().route_layout(topk_ids, int(num_experts), int(alignment), api._status_word(topk_ids.device)))
+
+
+def route_layout_masked(topk_ids: torch.Tensor, num_experts: int, max_rows: int) -> MaskedRouteLayout:
+    """As `route_layout` for the masked layout: expert e has the rows e * max_rows ... of [num_experts, max_rows]. Pairs that find
+    their expert's rows taken are dropped (row -1; first come, first served in token order), as a router with a capacity does."""
+    from . import api
+    return MaskedRouteLayout(*_lib.torch_ops().route_layout_masked(topk_ids, int(num_experts), int(max_rows), api._status_word(topk_ids.device)))

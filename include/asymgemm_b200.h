@@ -253,7 +253,8 @@ int ag_quant_rows_fp8(const void* x_bf16, void* q, float* sf, int64_t rows, int6
  * sf [rows, ceil(inter/128)] (activation of csrc/cpu/module.cpp:337-347 followed by the 1x128 quantiser). */
 int ag_silu_mul_quant_fp8(const void* gate_up_bf16, void* q, float* sf, int64_t rows, int64_t inter, int32_t pow2_scales, void* stream);
 
-/* dst[dst_rows ? dst_rows[i] : i] = src[src_rows ? src_rows[i] : i], i < rows; rows of row_bytes (multiple of 16) bytes. */
+/* dst[dst_rows ? dst_rows[i] : i] = src[src_rows ? src_rows[i] : i], i < rows; rows of row_bytes (multiple of 16) bytes. A
+ * negative dst_rows[i] writes nothing; a negative src_rows[i] writes zeros. */
 int ag_move_rows(const void* src, void* dst, const int64_t* src_rows, const int64_t* dst_rows, int64_t rows, int64_t row_bytes,
                  void* stream);
 
@@ -268,7 +269,7 @@ int ag_silu_mul_quant_fp8_upto(const void* gate_up_bf16, void* q, float* sf, int
                                const int32_t* rows_used, void* stream);
 
 /* y[t] = sum_j weights[t, j] * rows[pos[t * top_k + j]] accumulated in fp32, rounded once to bf16. cols % 8 == 0.
- * pos == NULL reads rows[t * top_k + j]. */
+ * pos == NULL reads rows[t * top_k + j]; slots with a negative pos add nothing. */
 int ag_combine_topk(const void* rows_bf16, const int64_t* pos, const float* weights, void* y_bf16, int64_t tokens, int32_t top_k,
                     int64_t cols, void* stream);
 
@@ -331,6 +332,124 @@ int ag_ep_dispatch(const void* x_q, const float* sfx, const int64_t* ids, int64_
 /* Every valid row of this rank's result `out` [cap_rows, row_bytes] is stored into its pair's slot of the source rank's `ret`. */
 int ag_ep_return(const void* out, const int64_t* my_meta, const int32_t* rows_used, int64_t cap_rows, int64_t row_bytes, int32_t world,
                  const ag_ep_peers_t* peers, void* stream);
+
+/* Routing of tokens to experts. Element types of tensors that come in several: */
+typedef enum ag_dtype { AG_T_BF16 = 0, AG_T_FP16 = 1, AG_T_FP32 = 2 } ag_dtype_t;
+typedef enum ag_score { AG_SCORE_SOFTMAX = 0, AG_SCORE_SIGMOID = 1 } ag_score_t;
+
+/* ids[t], weights[t] = the top_k experts of token t and their weights, from logits [tokens, experts] (rows `ld` apart).
+ *   score  s = softmax(l) over all experts, or sigmoid(l); choice c = s + bias (fp32 [experts], or NULL)
+ *   groups > 1: only the top_groups groups (of experts / groups consecutive experts) with the largest group score take part:
+ *           the sum of a group's two largest c, or its largest (group_max)
+ *   the top_k experts with the largest c, largest first, the lowest index among equals; without a bias: the largest logits
+ *   weight  s (without the bias), divided by the sum of the chosen s (renormalize), times scale
+ * The order is that of the formulas in exact arithmetic: experts whose fp32 scores are too close to tell are compared in fp64.
+ * A logit of NaN or -inf (or a bias of NaN or -inf) switches an expert off for the token, +inf counts as the largest
+ * finite number; slots for which no expert is left get id -1 and weight 0, and so do all slots of tokens from *rows_used (device
+ * int32, may be NULL) on. top_k <= 32; experts <= 1024 (one group; with several, 32 per lane of the 32 / groups lanes,
+ * rounded down to a power of two, that a group has). */
+typedef struct ag_route_desc {
+  const void* logits;
+  int64_t ld;              /* elements between rows of logits */
+  const float* bias;
+  const int32_t* rows_used;
+  int64_t* ids;            /* [tokens, top_k] */
+  float* weights;          /* [tokens, top_k] */
+  int64_t tokens;
+  int32_t dtype;           /* ag_dtype_t of the logits */
+  int32_t experts, top_k, groups, top_groups;
+  int32_t scoring;         /* ag_score_t */
+  int32_t group_max;
+  int32_t renormalize;
+  float scale;
+  void* stream;
+} ag_route_desc_t;
+int ag_route_topk(const ag_route_desc_t* desc);
+
+/* dlogits [tokens, experts] (type of the logits) from dweights [tokens, top_k] fp32, the ids ag_route_topk chose and its
+ * arguments; the choice itself and the bias have no gradient. Slots with an id outside [0, experts) add nothing. */
+int ag_route_topk_backward(const void* logits, int32_t dtype, int64_t tokens, int64_t ld, int32_t experts, const float* dweights, const int64_t* ids,
+                           int32_t top_k, int32_t scoring, int32_t renormalize, float scale, void* dlogits, void* stream);
+
+/* Tables of the grouped GEMM's layouts from ids [tokens, top_k] (int64 or int32; -1 = no expert; other ids outside
+ * [0, experts) count as -1 and set the status word). The pairs (token, slot) of an expert keep their order (a stable sort).
+ *   contiguous (max_rows 0): expert e's segment starts where the one before ends and is padded to a multiple of `alignment`
+ *     rows; offsets [2 * experts] = (start, end), expert_list [experts + 1] = 0 .. experts - 1, -1, rows_per_expert [experts].
+ *     rows (entries of row_token) must cover all segments: pairs + experts * (alignment - 1) is always enough.
+ *   masked (max_rows > 0): expert e has rows e * max_rows ...; masked_m [experts] = rows used; pairs past max_rows are dropped.
+ * pair_row [tokens * top_k] = the row of every pair, or -1; row_token [rows] = the token of every row, or -1. */
+typedef struct ag_route_layout_desc {
+  const void* ids;
+  int32_t ids_64;          /* ids are int64 (else int32) */
+  int32_t top_k;
+  int64_t tokens;
+  int32_t experts;         /* <= 1024 */
+  int32_t alignment;
+  int32_t max_rows;
+  int64_t rows;
+  int64_t* pair_row;
+  int64_t* row_token;
+  int64_t* rows_per_expert;
+  int32_t* offsets;
+  int32_t* expert_list;
+  int32_t* masked_m;
+  void* workspace;         /* ag_route_layout_workspace_bytes(tokens * top_k, experts) bytes, this call's alone while it runs */
+  uint64_t workspace_bytes;
+  int32_t* status;
+  void* stream;
+} ag_route_layout_desc_t;
+int ag_route_layout(const ag_route_layout_desc_t* desc);
+uint64_t ag_route_layout_workspace_bytes(int64_t pairs, int32_t experts);
+
+/* Gradient of ag_combine_topk / ag_combine_topk_f32: dweights [tokens, top_k] fp32 = <dy[t], rows[pos]> and drows [num_rows,
+ * cols] (type of rows) = weights[t, j] * dy[t] in row pos[t * top_k + j], 0 in rows that no pair names; either may be NULL.
+ * dy bf16 [tokens, cols]; rows, drows bf16 or fp32 (rows_fp32). pos entries outside [0, num_rows) add nothing; pos == NULL
+ * means t * top_k + j. With drows a row may be named once only: a second pair that names it sets the status word
+ * (AG_COMBINE_ROW_TWICE) and drows is then not the gradient. `row_seen` (with drows): num_rows bytes, rounded up to a multiple of 4, of this
+ * call's own. */
+#define AG_COMBINE_ROW_TWICE 66
+int ag_combine_topk_backward(const void* dy_bf16, const void* rows, int32_t rows_fp32, int64_t num_rows, const int64_t* pos, const float* weights,
+                             int64_t tokens, int32_t top_k, int64_t cols, void* drows, float* dweights, void* row_seen, int32_t* status,
+                             void* stream);
+
+/* Dense product with everything in its epilogue, weights in device memory (router logits, shared experts, projections):
+ *   z = x weight^T + bias,  y = act(z) + residual
+ * x [m, k], weight [n, k] bf16 or fp16, rows ldx / ldw elements apart on 16-byte boundaries, k a multiple of 8; bias [n] of their type or
+ * fp32, or NULL; y and residual [m, n] of their type or fp32 (out_dtype), rows ldy / ldr apart, residual may be NULL or y itself. `pre`
+ * (or NULL) receives z [m, n] in the operands' type, which the gradient of an activation needs. Accumulation in fp32, in runs
+ * of 512 terms on the tensor core joined by rounded fp32 additions; each output is rounded once.
+ * Gradients (ag_linear_backward): dz = dy act'(z), rounded to the operands' type for the products; dx [m, k] = dz weight and
+ * dweight [n, k] = dz^T x, contiguous, in the operands' type; dbias [n] = column sums of the unrounded dz, in bias_dtype. Any of
+ * the three may be NULL. dy [m, n] is of out_dtype, rows lddy apart; the gradient of the residual is dy itself. */
+typedef enum ag_activation { AG_ACT_NONE = 0, AG_ACT_RELU = 1, AG_ACT_GELU = 2 /* x Phi(x) */, AG_ACT_SILU = 3 } ag_activation_t;
+typedef struct ag_linear_desc {
+  int32_t dtype;       /* ag_dtype_t of x, weight, pre, dx, dweight */
+  int32_t out_dtype;   /* of y, residual, dy */
+  int32_t bias_dtype;  /* of bias, dbias */
+  int32_t activation;
+  int64_t m, n, k;
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* residual;
+  void* y;
+  void* pre;           /* written by ag_linear, read by ag_linear_backward */
+  int64_t ldx, ldw, ldr, ldy, ldp;
+  const void* dy;
+  int64_t lddy;
+  void* dx;
+  void* dweight;
+  void* dbias;
+  void* workspace;     /* 256-byte aligned, this call's alone while it runs */
+  uint64_t workspace_bytes;
+  int32_t* status;     /* device int32, as in ag_gemm_desc_t; NULL: the library's own */
+  uint32_t timeout_ms;
+  void* stream;
+} ag_linear_desc_t;
+int ag_linear(const ag_linear_desc_t* desc);
+int ag_linear_backward(const ag_linear_desc_t* desc);
+uint64_t ag_linear_backward_workspace_bytes(const ag_linear_desc_t* desc);
+uint64_t ag_linear_desc_size(void);
 
 /* Failure-detection self test: launches a one-CTA kernel whose only barrier wait can never be satisfied. After
  * `timeout_ms` (1..2000) the wait gives up, the kernel stores (0 << 8) | 9 ("wait-limit self test expired") in *status
