@@ -154,7 +154,7 @@ EXPORTS = [
     "ag_combine_topk_backward",
     "ag_linear",
     "ag_linear_backward",
-    "ag_linear_backward_workspace_bytes",
+    "ag_linear_workspace_bytes",
     "ag_linear_desc_size",
     "ag_gemm_desc_size",
     "ag_last_error",
@@ -255,8 +255,8 @@ def load() -> ctypes.CDLL:
     for name in ("ag_linear", "ag_linear_backward"):
         getattr(lib, name).argtypes = [POINTER(LinearDesc)]
         getattr(lib, name).restype = c_int32
-    lib.ag_linear_backward_workspace_bytes.argtypes = [POINTER(LinearDesc)]
-    lib.ag_linear_backward_workspace_bytes.restype = c_uint64
+    lib.ag_linear_workspace_bytes.argtypes = [POINTER(LinearDesc), c_int32]
+    lib.ag_linear_workspace_bytes.restype = c_uint64
     lib.ag_linear_desc_size.argtypes = []
     lib.ag_linear_desc_size.restype = c_uint64
     lib.ag_selftest_wait_limit.argtypes = [c_uint32, c_void_p, c_void_p]

@@ -21,9 +21,9 @@ constexpr int kDzCols = 256, kDzThreads = 256;
 
 __device__ __forceinline__ float slope(float z, int act) {
   if (act == ACT_RELU) return z > 0.f ? 1.f : z != z ? z : 0.f;
-  if (act == ACT_GELU) return normcdff(z) + z * 0.39894228f * expf(-0.5f * z * z);
+  if (act == ACT_GELU) return normal_cdf(z) + z * 0.39894228f * __expf(-0.5f * z * z);
   if (act == ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-z));
+    const float s = __fdividef(1.f, 1.f + __expf(-z));
     return s * (1.f + z * (1.f - s));
   }
   return 1.f;
@@ -137,43 +137,85 @@ struct Operand {
 };
 
 struct Plan {
+  bool pair;        // 256 x 256 tiles on pairs of CTAs, else 128 x bn tiles
   int bn, splits;
-  bool swapped;
+  bool swapped;     // tiles of 128 x bn: A and B change places
 };
 
-// Tile and split of a product. The narrower side is B, so that little of a tile is padding and the long side's rows (the
-// weights of a decode step) are spread over as many CTAs as possible; the contraction is split while the grid stays within
-// the CTAs that are resident at once and every split keeps four steps.
+// Tile and split of a product: the candidate that a simple model of its time (microseconds, fitted to a sweep over 54 shapes and 12
+// plans, see the figures beside it) finds fastest.
+//   pairs: a step takes 0.30 (0.28 is the tensor core's own time), a tile's epilogue 4.3 that overlaps the next tile's steps, a
+//   launch 5; split, the fp32 planes are written and read at about 4 TB/s by a second kernel.
+//   128 x bn: a step takes 0.21 (bn 16 .. 64) or 0.26 (128), limited by what an SM pulls out of L2, 1.6 times that where two
+//   CTAs share an SM; a launch and its epilogue 4.3 + bn / 64; joining s splits 0.35 s.
+// Measured at m, n, k (pairs / 128 x 128 / 128 x 64): 2048^3 17.5 / 28 / 26; 512, 2048, 2048 17.2 / 12.1 / 11.6; 128, 256, 7168
+// 39 / 12.8 / 10.2; 64, 7168, 2048 at bn 64, 32, 16: 10.0, 11.0, 12.9.
 Plan plan_product(const Operand& a, const Operand& b, int64_t steps, int sms) {
-  Plan pl{};
-  // the MN-major tile kernel exists for A alone, or for both
-  pl.swapped = a.mn == b.mn ? (!a.mn && a.rows <= 64 && b.rows > a.rows) : b.mn;
-  const int64_t ra = pl.swapped ? b.rows : a.rows, rb = pl.swapped ? a.rows : b.rows;
-  const bool both = a.mn && b.mn;
-  auto tiles = [&](int bn) { return (ra + agb::kTileA - 1) / agb::kTileA * ((rb + bn - 1) / bn); };
-  if (!both && rb <= 16) pl.bn = 16;
-  else if (!both && rb <= 32) pl.bn = 32;
-  else pl.bn = rb > 64 && tiles(128) >= sms ? 128 : 64;
-  const int64_t room = pl.bn == 128 ? sms : 2 * sms;
-  pl.splits = 1;
-  while (pl.splits < 8 && tiles(pl.bn) * pl.splits * 2 <= room && steps >= pl.splits * 2 * 4) pl.splits *= 2;
-  return pl;
+  Plan best{};
+  double best_us = 1e30;
+  auto consider = [&](const Plan& pl, double us) {
+    if (us < best_us) {
+      best = pl;
+      best_us = us;
+    }
+  };
+  auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+  const int64_t pair_tiles = up(a.rows, agb::kPairTile) * up(b.rows, agb::kPairTile);
+  for (int s = 1; s <= 8 && (s == 1 || steps >= 8 * s); ++s) {
+    const double waves = static_cast<double>(up(pair_tiles * s, sms / 2));
+    const double loop = 0.30 * static_cast<double>(up(steps, s));
+    const double join = s > 1 ? 3.0 + s * 8e-6 * static_cast<double>(a.rows) * static_cast<double>(b.rows) / 4.0 : 0.0;
+    consider({true, agb::kPairTile, s, false}, 5.0 + (waves - 1) * (loop > 4.3 ? loop : 4.3) + loop + 4.3 + join);
+  }
+  // 128 x bn tiles exist with A MN-major, or both operands, not B alone; of two K-major operands either may be A
+  for (int swapped = 0; swapped < 2; ++swapped) {
+    if (a.mn == b.mn ? (a.mn && swapped) : swapped != (b.mn ? 1 : 0)) continue;
+    const int64_t ra = swapped ? b.rows : a.rows, rb = swapped ? a.rows : b.rows;
+    for (int bn = a.mn && b.mn ? 64 : 16; bn <= 128; bn *= 2) {
+      if (!swapped && !b.mn && bn < 64) continue;      // rows of 16 outputs would be stored in 32-byte pieces
+      if (bn > 64 && rb <= bn / 2) continue;
+      const int64_t tiles = up(ra, agb::kTileA) * up(rb, bn);
+      for (int s = 1; s <= 8 && (s == 1 || steps >= 4 * s); s *= 2) {
+        const int64_t ctas = tiles * s;
+        const bool shared = bn < 128 && ctas > sms;
+        const double waves = static_cast<double>(up(ctas, bn < 128 ? 2 * sms : sms));
+        const double step = (bn < 128 ? 0.21 : 0.26) * (shared ? 1.6 : 1.0);
+        consider({false, bn, s, swapped != 0}, waves * (4.3 + bn / 64.0 + step * static_cast<double>(up(steps, s))) + (s > 1 ? 0.35 * s : 0.0));
+      }
+    }
+  }
+  return best;
+}
+
+template <typename K>
+cudaError_t allow_shared_memory(K kernel, int bytes, bool (&configured)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && configured[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+  return e;
+}
+
+template <bool A_MN, bool B_MN, bool ONE_CHUNK>
+cudaError_t launch_pair_as(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, int vector_width, int sms, cudaStream_t stream) {
+  auto kernel = agb::dense_pair_kernel<A_MN, B_MN, ONE_CHUNK>;
+  static bool configured[64] = {};
+  if (cudaError_t e = allow_shared_memory(kernel, agb::PairDenseSmem::dyn_bytes, configured)) return e;
+  const int64_t items = (static_cast<int64_t>(p.rows_a) + agb::kPairTile - 1) / agb::kPairTile * p.tiles_b * splits;
+  const int64_t pairs = sms / 2 < items ? sms / 2 : items;
+  kernel<<<static_cast<unsigned>(2 * pairs), agb::PAIR_THREADS, agb::PairDenseSmem::dyn_bytes, stream>>>(ma, mb, p, splits, vector_width);
+  return cudaGetLastError();
 }
 
 template <int BN, bool A_MN, bool B_MN>
-cudaError_t launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, cudaStream_t stream) {
+cudaError_t launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, int vector_width, cudaStream_t stream) {
   using L = agb::TileSmem<BN>;
   static_assert(L::dyn_bytes * (BN >= 128 ? 1 : 2) <= 232448, "tile configuration does not fit in shared memory");
   auto kernel = agb::dense_tile_kernel<BN, A_MN, B_MN>;
   static bool configured[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::dyn_bytes);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
+  if (cudaError_t e = allow_shared_memory(kernel, L::dyn_bytes, configured)) return e;
   const int64_t tiles = (static_cast<int64_t>(p.rows_a) + agb::kTileA - 1) / agb::kTileA * p.tiles_b;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -186,49 +228,106 @@ cudaError_t launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const agb:
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p, splits);
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, p, splits, vector_width);
 }
 
-// What goes into the epilogue; the rest of DenseParams follows from the operands.
-int run_product(Operand a, Operand b, int64_t k, int type, agb::DenseParams p, cudaStream_t stream) {
+int64_t steps_of(int64_t k) { return (k + agb::kStepK - 1) / agb::kStepK; }
+
+template <bool A_MN, bool B_MN>
+cudaError_t launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, int vector_width, int sms, cudaStream_t stream) {
+  return (p.steps + splits - 1) / splits <= p.chunk_steps ? launch_pair_as<A_MN, B_MN, true>(ma, mb, p, splits, vector_width, sms, stream)
+                                                          : launch_pair_as<A_MN, B_MN, false>(ma, mb, p, splits, vector_width, sms, stream);
+}
+
+// Bytes of partial results a product needs: one fp32 plane per split of the pair kernel.
+uint64_t product_workspace(const Operand& a, const Operand& b, int64_t k, int sms) {
+  const Plan pl = plan_product(a, b, steps_of(k), sms);
+  return pl.pair && pl.splits > 1 ? static_cast<uint64_t>(pl.splits) * a.rows * b.rows * 4 : 0;
+}
+
+// Columns a lane can write at once: rows of every output-shaped tensor aligned for them together.
+int vector_width(const agb::DenseParams& p, int64_t n) {
+  for (int vw = 4; vw > 1; vw /= 2) {
+    auto fits = [&](const void* base, int64_t ld, int type) {
+      const int64_t bytes = vw * (type == AG_T_FP32 ? 4 : 2);
+      return base == nullptr || (reinterpret_cast<uintptr_t>(base) % bytes == 0 && ld * (type == AG_T_FP32 ? 4 : 2) % bytes == 0);
+    };
+    if (n % vw == 0 && fits(p.out, p.ldo, p.out_type) && fits(p.residual, p.ldr, p.out_type) && fits(p.pre, p.ldp, p.pre_type)) return vw;
+  }
+  return 1;
+}
+
+template <int VW>
+void launch_join(const float* partial, int splits, const agb::DenseParams& p, cudaStream_t stream) {
+  const int64_t packs = static_cast<int64_t>(p.rows_a) * (p.rows_b / VW);
+  agb::join_splits_kernel<VW><<<static_cast<unsigned>((packs + 255) / 256), 256, 0, stream>>>(partial, splits, p);
+}
+
+// out[r, c] = sum_k a(r, k) b(c, k) with the epilogue that `p` names; the rest of DenseParams follows from the operands.
+int run_product(Operand a, Operand b, int64_t k, int type, agb::DenseParams p, void* workspace, cudaStream_t stream) {
   int sms = 0;
   if (int rc = agb_device_sm_count(&sms)) return rc;
-  const int64_t steps = (k + agb::kStepK - 1) / agb::kStepK;
-  const Plan pl = plan_product(a, b, steps, sms);
+  const Plan pl = plan_product(a, b, steps_of(k), sms);
   if (pl.swapped) {
     const Operand t = a;
     a = b;
     b = t;
   }
-  CUtensorMap ma, mb;
-  auto encode = [&](CUtensorMap* map, const Operand& o, int tile_rows) {
+  auto encode = [&](CUtensorMap* map, const Operand& o, int box_rows) {
     return o.mn ? agb_encode_16bit_2d(map, o.p, static_cast<uint64_t>(o.rows), static_cast<uint64_t>(k), static_cast<uint64_t>(o.ld) * 2, agb::kStepK, o.what)
                 : agb_encode_16bit_2d(map, o.p, static_cast<uint64_t>(k), static_cast<uint64_t>(o.rows), static_cast<uint64_t>(o.ld) * 2,
-                                      static_cast<uint32_t>(tile_rows), o.what);
+                                      static_cast<uint32_t>(box_rows), o.what);
   };
+  CUtensorMap ma, mb;
   if (int rc = encode(&ma, a, agb::kTileA)) return rc;
-  if (int rc = encode(&mb, b, pl.bn)) return rc;
+  if (int rc = encode(&mb, b, pl.pair ? 128 : pl.bn)) return rc;
   p.rows_a = static_cast<int>(a.rows);
   p.rows_b = static_cast<int>(b.rows);
-  p.steps = static_cast<int>(steps);
+  p.steps = static_cast<int>(steps_of(k));
+  p.chunk_steps = p.out_type == AG_T_FP32 ? agb::kChunkStepsFp32 : agb::kChunkSteps16Bit;
   p.tiles_b = static_cast<int>((b.rows + pl.bn - 1) / pl.bn);
   p.swapped = pl.swapped;
   // operand format 0 = fp16, 1 = bf16; bits 15 and 16: A, B are MN-major
-  p.idesc = agb::make_idesc(1, type == AG_T_BF16 ? 1u : 0u, static_cast<uint32_t>(pl.bn)) | (a.mn ? 1u << 15 : 0u) | (b.mn ? 1u << 16 : 0u);
+  const uint32_t format = type == AG_T_BF16 ? 1u : 0u;
+  p.idesc = (pl.pair ? agb::make_idesc_pair(1, format, agb::kPairTile) : agb::make_idesc(1, format, static_cast<uint32_t>(pl.bn))) |
+            (a.mn ? 1u << 15 : 0u) | (b.mn ? 1u << 16 : 0u);
   cudaError_t e = cudaErrorInvalidValue;
-  if (!a.mn && !b.mn) {
-    if (pl.bn == 16) e = launch_tile<16, false, false>(ma, mb, p, pl.splits, stream);
-    else if (pl.bn == 32) e = launch_tile<32, false, false>(ma, mb, p, pl.splits, stream);
-    else if (pl.bn == 64) e = launch_tile<64, false, false>(ma, mb, p, pl.splits, stream);
-    else e = launch_tile<128, false, false>(ma, mb, p, pl.splits, stream);
+  const int64_t out_cols = pl.swapped ? a.rows : b.rows;
+  int vw = vector_width(p, out_cols);
+  if (pl.pair) {
+    agb::DenseParams q = p;
+    if (pl.splits > 1) {      // raw partials now, the epilogue when they are joined
+      q.bias = q.residual = nullptr;
+      q.pre = nullptr;
+      q.act = agb::ACT_NONE;
+      q.out = workspace;
+      q.ldo = b.rows;
+      q.out_type = AG_T_FP32;
+    }
+    const int join_vw = vw;
+    vw = vector_width(q, out_cols);
+    if (!a.mn && !b.mn) e = launch_pair<false, false>(ma, mb, q, pl.splits, vw, sms, stream);
+    else if (!a.mn) e = launch_pair<false, true>(ma, mb, q, pl.splits, vw, sms, stream);
+    else if (b.mn) e = launch_pair<true, true>(ma, mb, q, pl.splits, vw, sms, stream);
+    if (e == cudaSuccess && pl.splits > 1) {
+      if (join_vw == 4) launch_join<4>(static_cast<const float*>(workspace), pl.splits, p, stream);
+      else if (join_vw == 2) launch_join<2>(static_cast<const float*>(workspace), pl.splits, p, stream);
+      else launch_join<1>(static_cast<const float*>(workspace), pl.splits, p, stream);
+      e = cudaGetLastError();
+    }
+  } else if (!a.mn && !b.mn) {
+    if (pl.bn == 16) e = launch_tile<16, false, false>(ma, mb, p, pl.splits, vw, stream);
+    else if (pl.bn == 32) e = launch_tile<32, false, false>(ma, mb, p, pl.splits, vw, stream);
+    else if (pl.bn == 64) e = launch_tile<64, false, false>(ma, mb, p, pl.splits, vw, stream);
+    else e = launch_tile<128, false, false>(ma, mb, p, pl.splits, vw, stream);
   } else if (!b.mn) {
-    if (pl.bn == 16) e = launch_tile<16, true, false>(ma, mb, p, pl.splits, stream);
-    else if (pl.bn == 32) e = launch_tile<32, true, false>(ma, mb, p, pl.splits, stream);
-    else if (pl.bn == 64) e = launch_tile<64, true, false>(ma, mb, p, pl.splits, stream);
-    else e = launch_tile<128, true, false>(ma, mb, p, pl.splits, stream);
+    if (pl.bn == 16) e = launch_tile<16, true, false>(ma, mb, p, pl.splits, vw, stream);
+    else if (pl.bn == 32) e = launch_tile<32, true, false>(ma, mb, p, pl.splits, vw, stream);
+    else if (pl.bn == 64) e = launch_tile<64, true, false>(ma, mb, p, pl.splits, vw, stream);
+    else e = launch_tile<128, true, false>(ma, mb, p, pl.splits, vw, stream);
   } else {
-    if (pl.bn == 64) e = launch_tile<64, true, true>(ma, mb, p, pl.splits, stream);
-    else e = launch_tile<128, true, true>(ma, mb, p, pl.splits, stream);
+    if (pl.bn == 64) e = launch_tile<64, true, true>(ma, mb, p, pl.splits, vw, stream);
+    else e = launch_tile<128, true, true>(ma, mb, p, pl.splits, vw, stream);
   }
   return e == cudaSuccess ? AG_OK : agb_fail(AG_E_CUDA, cudaGetErrorString(e));
 }
@@ -262,14 +361,28 @@ int64_t dz_rows(const ag_linear_desc_t* g) {
   return (rows < 8 ? 8 : rows + 7) / 8 * 8;
 }
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+// The three products; dz [m, n] with rows `ld` apart.
+Operand x_rows(const ag_linear_desc_t* g) { return {g->x, g->ldx, g->m, false, "x"}; }
+Operand weight_rows(const ag_linear_desc_t* g) { return {g->weight, g->ldw, g->n, false, "weight"}; }
+Operand weight_columns(const ag_linear_desc_t* g) { return {g->weight, g->ldw, g->k, true, "weight"}; }
+Operand x_columns(const ag_linear_desc_t* g) { return {g->x, g->ldx, g->k, true, "x"}; }
+Operand dz_by_row(const ag_linear_desc_t* g, const void* dz, int64_t ld) { return {dz, ld, g->m, false, "dz"}; }
+Operand dz_by_column(const ag_linear_desc_t* g, const void* dz, int64_t ld) { return {dz, ld, g->n, true, "dz"}; }
+
 struct BackwardSpace {
-  uint64_t dz, partial, total;
+  uint64_t dz, partial, product, total;     // product: shared by the two products, which run one after the other
 };
-BackwardSpace backward_space(const ag_linear_desc_t* g) {
+BackwardSpace backward_space(const ag_linear_desc_t* g, int sms) {
   BackwardSpace s{};
   if (needs_dz(g) && (g->dx != nullptr || g->dweight != nullptr)) s.dz = align256(static_cast<uint64_t>(g->m) * dz_ld(g) * 2);
   if (g->dbias != nullptr) s.partial = align256(static_cast<uint64_t>((g->m + dz_rows(g) - 1) / dz_rows(g)) * g->n * 4);
-  s.total = s.dz + s.partial;
+  if (g->dx != nullptr) s.product = product_workspace(dz_by_row(g, nullptr, 0), weight_columns(g), g->n, sms);
+  if (g->dweight != nullptr) {
+    const uint64_t need = product_workspace(dz_by_column(g, nullptr, 0), x_columns(g), g->m, sms);
+    if (need > s.product) s.product = need;
+  }
+  s.total = s.dz + s.partial + s.product;
   return s;
 }
 
@@ -308,11 +421,19 @@ int ag_linear(const ag_linear_desc_t* g) {
   p.ldp = g->ldp;
   p.pre_type = g->dtype;
   p.act = g->activation;
-  return run_product({g->x, g->ldx, g->m, false, "x"}, {g->weight, g->ldw, g->n, false, "weight"}, g->k, g->dtype, p,
-                     static_cast<cudaStream_t>(g->stream));
+  int sms = 0;
+  if (int rc = agb_device_sm_count(&sms)) return rc;
+  const uint64_t need = product_workspace(x_rows(g), weight_rows(g), g->k, sms);
+  if (need > 0 && (g->workspace == nullptr || g->workspace_bytes < need || !aligned_to(g->workspace, 256)))
+    return agb_fail(AG_E_INVALID, "workspace too small or not 256-byte aligned (ag_linear_workspace_bytes)");
+  return run_product(x_rows(g), weight_rows(g), g->k, g->dtype, p, g->workspace, static_cast<cudaStream_t>(g->stream));
 }
 
-uint64_t ag_linear_backward_workspace_bytes(const ag_linear_desc_t* g) { return g == nullptr || g->m <= 0 || g->n <= 0 ? 0 : backward_space(g).total; }
+uint64_t ag_linear_workspace_bytes(const ag_linear_desc_t* g, int32_t backward) {
+  int sms = 0;
+  if (check_common(g) != AG_OK || g->m == 0 || agb_device_sm_count(&sms) != AG_OK) return 0;
+  return backward ? backward_space(g, sms).total : product_workspace(x_rows(g), weight_rows(g), g->k, sms);
+}
 
 int ag_linear_backward(const ag_linear_desc_t* g) {
   if (int rc = check_common(g)) return rc;
@@ -330,9 +451,11 @@ int ag_linear_backward(const ag_linear_desc_t* g) {
   if (g->activation != AG_ACT_NONE && g->pre == nullptr) return agb_fail(AG_E_INVALID, "the gradient of an activation wants `pre` of the forward call");
   if (g->lddy < g->n || (g->pre != nullptr && g->ldp < g->n)) return agb_fail(AG_E_INVALID, "rows of dy and pre must not overlap");
   if (!aligned_to(g->dy, size_of(g->out_dtype)) || !aligned_to(g->pre, 2)) return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
-  const BackwardSpace space = backward_space(g);
+  int sms = 0;
+  if (int rc = agb_device_sm_count(&sms)) return rc;
+  const BackwardSpace space = backward_space(g, sms);
   if (space.total > 0 && (g->workspace == nullptr || g->workspace_bytes < space.total || !aligned_to(g->workspace, 256)))
-    return agb_fail(AG_E_INVALID, "workspace too small or not 256-byte aligned (ag_linear_backward_workspace_bytes)");
+    return agb_fail(AG_E_INVALID, "workspace too small or not 256-byte aligned (ag_linear_workspace_bytes)");
 
   const void* dz = g->dy;
   int64_t ld = g->lddy;
@@ -364,15 +487,16 @@ int ag_linear_backward(const ag_linear_desc_t* g) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   }
+  void* product_space = static_cast<char*>(g->workspace) + space.dz + space.partial;
   if (g->dx != nullptr) {      // dx[m, k] = sum_n dz[m, n] W[n, k]
     agb::DenseParams p = plain_output(g, g->dx, g->k, g->dtype);
     if (p.status == nullptr) return agb_fail(AG_E_CUDA, "no status word");
-    if (int rc = run_product({dz, ld, g->m, false, "dz"}, {g->weight, g->ldw, g->k, true, "weight"}, g->n, g->dtype, p, stream)) return rc;
+    if (int rc = run_product(dz_by_row(g, dz, ld), weight_columns(g), g->n, g->dtype, p, product_space, stream)) return rc;
   }
   if (g->dweight != nullptr) {      // dW[n, k] = sum_m dz[m, n] x[m, k]
     agb::DenseParams p = plain_output(g, g->dweight, g->k, g->dtype);
     if (p.status == nullptr) return agb_fail(AG_E_CUDA, "no status word");
-    if (int rc = run_product({dz, ld, g->n, true, "dz"}, {g->x, g->ldx, g->k, true, "x"}, g->m, g->dtype, p, stream)) return rc;
+    if (int rc = run_product(dz_by_column(g, dz, ld), x_columns(g), g->m, g->dtype, p, product_space, stream)) return rc;
   }
   return AG_OK;
 }

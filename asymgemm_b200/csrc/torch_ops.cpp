@@ -306,6 +306,17 @@ ag_linear_desc_t linear_desc(const at::Tensor& x, const at::Tensor& weight, int6
   return d;
 }
 
+at::Tensor linear_workspace(ag_linear_desc_t& d, const at::Tensor& x, bool backward) {
+  at::Tensor workspace;
+  const uint64_t need = ag_linear_workspace_bytes(&d, backward);
+  if (need > 0) {
+    workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+    d.workspace = workspace.data_ptr();
+    d.workspace_bytes = need;
+  }
+  return workspace;
+}
+
 std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, int64_t activation,
                                           const OptTensor& residual, bool out_fp32, bool keep_pre, const at::Tensor& status, int64_t timeout_ms) {
   ag_linear_desc_t d = linear_desc(x, weight, activation, status, timeout_ms);
@@ -334,6 +345,7 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
     d.pre = pre.data_ptr();
     d.ldp = d.n;
   }
+  const at::Tensor workspace = linear_workspace(d, x, false);
   d.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   check_ok(ag_linear(&d));
   return {y, pre};
@@ -371,12 +383,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
     d.bias_dtype = bias_fp32 ? AG_T_FP32 : d.dtype;
     d.dbias = dbias.data_ptr();
   }
-  const uint64_t need = ag_linear_backward_workspace_bytes(&d);
-  if (need > 0) {
-    workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
-    d.workspace = workspace.data_ptr();
-    d.workspace_bytes = need;
-  }
+  workspace = linear_workspace(d, x, true);
   d.stream = c10::cuda::getCurrentCUDAStream(x.device().index()).stream();
   check_ok(ag_linear_backward(&d));
   return {dx, dweight, dbias};

@@ -448,7 +448,8 @@ typedef struct ag_linear_desc {
 } ag_linear_desc_t;
 int ag_linear(const ag_linear_desc_t* desc);
 int ag_linear_backward(const ag_linear_desc_t* desc);
-uint64_t ag_linear_backward_workspace_bytes(const ag_linear_desc_t* desc);
+/* workspace_bytes the call will want on the current device (backward: ag_linear_backward); 0 for a descriptor it would refuse. */
+uint64_t ag_linear_workspace_bytes(const ag_linear_desc_t* desc, int32_t backward);
 uint64_t ag_linear_desc_size(void);
 
 /* Failure-detection self test: launches a one-CTA kernel whose only barrier wait can never be satisfied. After
