@@ -13,6 +13,7 @@
 #include "../../include/asymgemm_b200.h"
 
 int agb_fail(int code, const char* message);
+int agb_device_sm_count(int* out);
 
 namespace agb {
 
@@ -55,7 +56,7 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 }
 
 // A logit as the router counts it: NaN and -inf switch the expert off, +inf is the largest finite number.
-__device__ __forceinline__ float clean(float l) { return l != l ? -INFINITY : fminf(l, FLT_MAX); }
+__device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINITY), FLT_MAX); }   // max(NaN, x) = x
 
 struct RouteParams {
   const void* logits;
@@ -64,25 +65,28 @@ struct RouteParams {
   long long* ids;
   float* weights;
   long long tokens, ld;
-  int experts, top_k, groups, top_groups, group_size, lanes_per_group, per_lane;
+  int experts, top_k, groups, top_groups, group_size, lanes_per_group, lane_shift, per_lane;   // lanes_per_group = 1 << lane_shift
   int sigmoid, group_max, renormalize, vector_rows;
   float scale;
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-// One warp per token. The experts of a group lie on `lanes_per_group` (a power of two) neighbouring lanes, `per_lane`
-// consecutive ones each, so the lane order is the expert order, a group's two best scores are a short shuffle
-// reduction, and "lowest index among equals" is "lowest lane, then lowest slot". The k best are taken one at a time: a
-// warp-wide maximum of the lanes' own maxima (one redux), the first lane that holds it gives its expert up.
+// One warp per token, persistent over tokens with the next row's load under way. The experts of a group lie on
+// `lanes_per_group` (a power of two) neighbouring lanes, `per_lane` consecutive ones each, so the lane order is the expert
+// order, a group's two best scores are a short shuffle reduction, and "lowest index among equals" is "lowest lane, then lowest
+// slot". Each lane sorts its experts once (lists of 8, as 32-bit keys that carry the slot in their lowest bits); the k best are
+// then taken off the heads of the lists, one warp-wide integer maximum and one predicated shift each: about 17 instructions
+// per expert where searching the lane's slots again took 60. With 256 experts the kernel executes some 500 instructions per
+// KB of logits and is bound by their issue, not by memory (65536 tokens: see the figures at launch_route).
 //
-// Order. With neither bias nor groups the experts are ordered by their logits, which are exact. Otherwise two experts
-// (or two groups) whose fp32 scores are closer than fp32 resolves could come out in either order; `tol` bounds what the
-// fp32 scores are off by, and a token with two neighbours inside it -- one in a thousand -- is decided once more in 64 bits
-// (route_exact), so that the result is that of the formulas whatever the last bits of expf are.
+// Order. Keys are scores in fp32, cut off at the slot bits; `tol` bounds what they are off by. A token with two neighbours in
+// the order, or two groups at the border, closer than that -- one in a few hundred -- is decided once more in 64 bits
+// (route_exact), unless the two have equal logits and biases, whose order is by index in any arithmetic. The result is that of
+// the formulas whatever the last bits of the exponentials are.
 struct Slots {
   int first, count;      // this lane holds the experts first .. first + count - 1
   __device__ __forceinline__ Slots(const RouteParams& p, int lane) {
-    const int g = lane / p.lanes_per_group, in = (lane % p.lanes_per_group) * p.per_lane;
+    const int g = lane >> p.lane_shift, in = (lane & (p.lanes_per_group - 1)) * p.per_lane;
     first = g * p.group_size + in;
     count = g < p.groups ? max(0, min(p.per_lane, p.group_size - in)) : 0;
   }
@@ -128,7 +132,7 @@ __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int 
       a1 = fmax(a1, b1);
     }
     const double mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
-    const int g = lane / p.lanes_per_group;
+    const int g = lane >> p.lane_shift;
     int rank = 0;
     for (int o = 0; o < p.groups; ++o) {
       const double other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
@@ -190,150 +194,235 @@ __device__ __forceinline__ void load_slots(const RouteParams& p, const T* row, c
   for (int j = 0; j < VPL; ++j) l[j] = j < at.count ? clean(to_float(row[at.first + j])) : -INFINITY;
 }
 
+// Order-preserving map of floats to signed integers (its own inverse). -inf, "off", maps below every live key.
+__device__ __forceinline__ int32_t key_of(float v) {
+  const int32_t u = __float_as_int(v + 0.f);        // -0 and 0 are equal
+  return u ^ ((u >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float value_of(int32_t key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
+constexpr int32_t kOffKeys = static_cast<int32_t>(0x807fffffu);      // keys of -inf with any slot bits are not above this
+
+__device__ __forceinline__ void order(int32_t& a, int32_t& b) {
+  const int32_t hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+// Batcher's odd-even merge sort, largest first.
+template <int N>
+__device__ __forceinline__ void sort_list(int32_t (&s)[N]) {
+  if constexpr (N >= 2) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) order(s[i], s[i + 1]);
+  }
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      order(s[i], s[i + 2]);
+      order(s[i + 1], s[i + 3]);
+      order(s[i + 1], s[i + 2]);
+    }
+  }
+  if constexpr (N == 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) order(s[i], s[i + 4]);
+    order(s[2], s[4]);
+    order(s[3], s[5]);
+    order(s[1], s[2]);
+    order(s[3], s[4]);
+    order(s[5], s[6]);
+  }
+}
+
 template <typename T, int VPL>
 __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
-  const long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  constexpr int kLen = VPL < 8 ? VPL : 8, kLists = VPL / kLen;
+  constexpr int32_t kSlotMask = VPL - 1;      // key bits that hold VPL - 1 - slot
   const int lane = threadIdx.x & 31;
-  if (token >= p.tokens) return;
-  long long* ids = p.ids + token * p.top_k;
-  float* weights = p.weights + token * p.top_k;
-  if (p.rows_used != nullptr && token >= *p.rows_used) {      // a padding token is routed nowhere
-    if (lane < p.top_k) {
-      ids[lane] = -1;
-      weights[lane] = 0.f;
-    }
-    return;
-  }
-  const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+  const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
+  const long long used = p.rows_used != nullptr ? *p.rows_used : p.tokens;
   const bool scored = p.bias != nullptr || p.groups > 1;      // the order needs the scores, not just the logits
-
   const Slots at(p, lane);
-  float c[VPL];      // what the experts are ordered by; -inf = off or taken
-  load_slots<T, VPL>(p, row, at, c);
-  float mx = c[0];
+  float bias[VPL];
+  if (p.bias != nullptr) {
 #pragma unroll
-  for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
-  float row_max = 0.f, sum = 0.f;
-  if (!p.sigmoid && (scored || !p.renormalize)) {
-    row_max = warp_max_f(mx);
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? expf(c[j] - row_max) : 0.f;
-    sum = warp_sum_f(sum);
+    for (int j = 0; j < VPL; ++j) bias[j] = j < at.count ? clean(__ldg(p.bias + at.first + j)) : -INFINITY;
   }
-  bool unsure = false;
-  float tol = 0.f;
-  if (scored) {
-    float s[VPL];
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      if (p.sigmoid) s[j] = 1.f / (1.f + expf(-c[j]));
-      else s[j] = expf(c[j] - row_max) * inv;
-      if (c[j] == -INFINITY) s[j] = -INFINITY;
-    }
-    // Error of a score: sigmoid, below 8 roundings of a number <= 1; softmax, of numbers <= 1 / sum: the argument's
-    // rounding, d e^-d 2^-24 at most for l = max - d, and up to 37 additions in the sum. A bias adds half a step of the result.
-    tol = p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;
-    if (p.bias != nullptr) {
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const float b = j < at.count ? clean(__ldg(p.bias + at.first + j)) : -INFINITY;
-        s[j] = s[j] == -INFINITY || b == -INFINITY ? -INFINITY : s[j] + b;
-      }
-    }
-    if (p.groups > 1) {
-      float a1 = -INFINITY, a2 = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        a2 = fmaxf(a2, fminf(a1, s[j]));
-        a1 = fmaxf(a1, s[j]);
-      }
-      for (int o = 1; o < p.lanes_per_group; o <<= 1) {
-        const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
-        a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
-        a1 = fmaxf(a1, b1);
-      }
-      const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
-      const int g = lane / p.lanes_per_group;
-      int rank = 0;
-      for (int o = 0; o < p.groups; ++o) {
-        const float other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
-        rank += other > mine || (other == mine && o < g);
-      }
-      const bool kept = rank < p.top_groups;
-      const bool real = g < p.groups;
-      // the weakest group kept against the strongest one left out
-      const float low = -warp_max_f(real && kept ? -mine : -INFINITY), high = warp_max_f(real && !kept ? mine : -INFINITY);
-      if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
-      if (!kept) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = c[j] = -INFINITY;
-      }
-    }
-    if (p.bias != nullptr) {
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) c[j] = s[j];
-    }
-    mx = c[0];
-#pragma unroll
-    for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
-  }
+  long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  float next[VPL];
+  if (token < min(used, p.tokens)) load_slots<T, VPL>(p, static_cast<const T*>(p.logits) + token * p.ld, at, next);
 
-  int chosen = -1;
-  float last = 0.f;
-  int last_e = 0;
-  const int rounds = p.bias != nullptr ? p.top_k + 1 : p.top_k;    // one more, to see how far the first one left out is
-  for (int i = 0; i < rounds && !unsure; ++i) {
-    const float best = warp_max_f(mx);
-    if (best == -INFINITY) break;
-    const int w = __ffs(__ballot_sync(kAll, mx == best)) - 1;
-    int e = -1;
-    if (lane == w) {
-      mx = -INFINITY;
+  for (; token < p.tokens; token += warps) {
+    long long* ids = p.ids + token * p.top_k;
+    float* weights = p.weights + token * p.top_k;
+    if (token >= used) {      // a padding token is routed nowhere
+      if (lane < p.top_k) {
+        ids[lane] = -1;
+        weights[lane] = 0.f;
+      }
+      continue;
+    }
+    const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+    float c[VPL];      // what the experts are ordered by; -inf = off
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) c[j] = next[j];
+    if (token + warps < min(used, p.tokens)) load_slots<T, VPL>(p, row + warps * p.ld, at, next);
+
+    float row_max = 0.f, sum = 0.f;
+    if (!p.sigmoid && (scored || !p.renormalize)) {
+      float mx = c[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
+      row_max = warp_max_f(mx);
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? __expf(c[j] - row_max) : 0.f;
+      sum = warp_sum_f(sum);
+    }
+    bool unsure = false;
+    float tol = 0.f;
+    if (scored) {
+      float s[VPL];
+      const float inv = 1.f / sum;
 #pragma unroll
       for (int j = 0; j < VPL; ++j) {
-        if (e < 0 && c[j] == best) {
-          e = at.first + j;
-          c[j] = -INFINITY;
+        s[j] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[j])) : __expf(c[j] - row_max) * inv;
+      }
+      bool any_off = false;      // rare, so the common row has no select per expert
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) any_off = any_off || c[j] == -INFINITY;
+      // Error of a score. Sigmoid: s (1 - s) |l| 2^-23 from the exponential's argument, a few roundings of a number <= 1.
+      // Softmax, of numbers <= 1 / sum: d e^-d 2^-23 for l = max - d, and up to 37 additions in the sum.
+      tol = p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) s[j] += bias[j];      // a bias of -inf switches the expert off by itself
+      }
+      if (any_off) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+      }
+      if (p.groups > 1) {
+        float a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+          a2 = fmaxf(a2, fminf(a1, s[j]));
+          a1 = fmaxf(a1, s[j]);
         }
-        mx = fmaxf(mx, c[j]);
+        for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+          const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+          a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
+          a1 = fmaxf(a1, b1);
+        }
+        const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
+        const int g = lane >> p.lane_shift;
+        int rank = 0;
+        for (int o = 0; o < p.groups; ++o) {
+          const float other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
+          rank += other > mine || (other == mine && o < g);
+        }
+        const bool kept = rank < p.top_groups, real = g < p.groups;
+        // the weakest group kept against the strongest one left out
+        const float low = -warp_max_f(real && kept ? -mine : -INFINITY), high = warp_max_f(real && !kept ? mine : -INFINITY);
+        if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
+        if (!kept) {
+#pragma unroll
+          for (int j = 0; j < VPL; ++j) s[j] = c[j] = -INFINITY;
+        }
+      }
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) c[j] = s[j];
       }
     }
-    e = __shfl_sync(kAll, e, w);
-    if (p.bias != nullptr) {
-      if (i > 0 && !(last - best > 2.f * tol + 0x1p-21f * (fabsf(last) + fabsf(best))))
-        // equal logits with equal biases are equal whatever the arithmetic: lowest index first, as taken here
-        unsure = last != best || clean(to_float(row[e])) != clean(to_float(row[last_e])) || clean(p.bias[e]) != clean(p.bias[last_e]);
-      last = best;
-      last_e = e;
-    }
-    if (lane == i) chosen = e;
-  }
-  if (lane >= p.top_k) chosen = -1;
-  if (unsure) chosen = route_exact<T, VPL>(p, row, lane);
 
-  // Weights, lane i for the expert chosen i-th. Sums over at most 32 chosen experts, in fp32.
-  const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
-  float w = 0.f;
-  if (p.renormalize) {
-    // scores up to a common factor: shifting by the largest chosen logit (sigmoid: only where all are negative) keeps
-    // rows of very small scores away from 0 / 0
-    float top = warp_max_f(l);
-    if (p.sigmoid) {
-      top = fminf(top, 0.f);
-      w = l >= 0.f ? 1.f / (1.f + expf(-l)) : expf(l - top) / (1.f + expf(l));
-    } else {
-      w = expf(l - top);
+    int32_t list[kLists][kLen];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) list[j / kLen][j % kLen] = (key_of(c[j]) & ~kSlotMask) | (VPL - 1 - j);
+#pragma unroll
+    for (int q = 0; q < kLists; ++q) sort_list<kLen>(list[q]);
+
+    int32_t my_key = kOffKeys;      // lane i: the key and lane of the expert taken i-th
+    int my_lane = 0;
+    auto head = [&] {
+      int32_t h = list[0][0];
+#pragma unroll
+      for (int q = 1; q < kLists; ++q) h = max(h, list[q][0]);
+      return h;
+    };
+    // The best head by value, of equal ones the lowest lane's (the slot bits order experts within a lane only).
+    auto take_best = [&](int32_t h, int& w) {
+      const int32_t value = __reduce_max_sync(kAll, h & ~kSlotMask);
+      w = __ffs(__ballot_sync(kAll, (h & ~kSlotMask) == value)) - 1;
+      return __shfl_sync(kAll, h, w);
+    };
+    for (int i = 0; i < p.top_k; ++i) {
+      int w;
+      const int32_t best = take_best(head(), w);
+      if (best <= kOffKeys) break;
+#pragma unroll
+      for (int q = 0; q < kLists; ++q) {
+        const bool pop = lane == w && list[q][0] == best;
+#pragma unroll
+        for (int j = 0; j + 1 < kLen; ++j) list[q][j] = pop ? list[q][j + 1] : list[q][j];
+        list[q][kLen - 1] = pop ? INT32_MIN : list[q][kLen - 1];
+      }
+      if (lane == i) {
+        my_key = best;
+        my_lane = w;
+      }
     }
-    if (chosen < 0) w = 0.f;
-    const float total = warp_sum_f(w);
-    w = chosen >= 0 ? w / total : 0.f;
-  } else if (chosen >= 0) {
-    w = p.sigmoid ? 1.f / (1.f + expf(-l)) : expf(l - row_max) / sum;
-  }
-  if (lane < p.top_k) {
-    ids[lane] = chosen;
-    weights[lane] = w * p.scale;
+    auto expert_of = [&](int32_t key, int owner) {
+      const int g = owner >> p.lane_shift, in = (owner & (p.lanes_per_group - 1)) * p.per_lane;
+      return key <= kOffKeys ? -1 : g * p.group_size + in + kSlotMask - (key & kSlotMask);
+    };
+    int chosen = expert_of(my_key, my_lane);
+    {
+      // each expert taken against the next in the order: lane top_k - 1's next is the first one left out
+      int out_lane;
+      const int32_t out = take_best(head(), out_lane);
+      int32_t next_key = __shfl_down_sync(kAll, my_key, 1);
+      int next_e = __shfl_down_sync(kAll, chosen, 1);
+      if (lane == p.top_k - 1) {
+        next_key = out;
+        next_e = expert_of(out, out_lane);
+      }
+      const float v = value_of(my_key & ~kSlotMask), u = value_of(next_key & ~kSlotMask);
+      constexpr float kCut = VPL * 0x1p-23f + 0x1p-22f;      // the slot bits cut off, half a step of the sum with the bias
+      const float off = p.bias != nullptr ? tol : 0.f;
+      bool close = lane < p.top_k && my_key > kOffKeys && next_key > kOffKeys && !(v - u > 2.f * off + kCut * (fabsf(v) + fabsf(u)));
+      if (__any_sync(kAll, close)) {
+        if (close) {
+          close = clean(to_float(row[chosen])) != clean(to_float(row[next_e])) ||
+                  (p.bias != nullptr && clean(p.bias[chosen]) != clean(p.bias[next_e]));
+        }
+        unsure = unsure || __any_sync(kAll, close);
+      }
+    }
+    if (unsure) chosen = route_exact<T, VPL>(p, row, lane);
+
+    // Weights, lane i for the expert chosen i-th. Sums over at most 32 chosen experts, in fp32.
+    const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
+    float w = 0.f;
+    if (p.renormalize) {
+      // scores up to a common factor: shifting by the largest chosen logit (sigmoid: only where all are negative) keeps
+      // rows of very small scores away from 0 / 0
+      float top = warp_max_f(l);
+      if (p.sigmoid) {
+        top = fminf(top, 0.f);
+        const float t = __expf(-fabsf(l));
+        w = __fdividef(l >= 0.f ? 1.f : __expf(l - top), 1.f + t);
+      } else {
+        w = __expf(l - top);
+      }
+      if (chosen < 0) w = 0.f;
+      const float total = warp_sum_f(w);
+      w = chosen >= 0 ? __fdividef(w, total) : 0.f;
+    } else if (chosen >= 0) {
+      w = __fdividef(p.sigmoid ? 1.f : __expf(l - row_max), p.sigmoid ? 1.f + __expf(-l) : sum);
+    }
+    if (lane < p.top_k) {
+      ids[lane] = chosen;
+      weights[lane] = w * p.scale;
+    }
   }
 }
 
@@ -621,16 +710,20 @@ int launch_check() {
 bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 int size_of(int dtype) { return dtype == AG_T_FP32 ? 4 : 2; }
 
+template <typename T, int VPL>
+void launch_route_as(const agb::RouteParams& p, int sms, cudaStream_t stream) {
+  constexpr int kWarps = 4, kBlocksPerSm = VPL <= 8 ? 8 : VPL == 16 ? 6 : 4;
+  const long long blocks = (p.tokens + kWarps - 1) / kWarps, most = static_cast<long long>(sms) * kBlocksPerSm;
+  agb::route_topk_kernel<T, VPL><<<static_cast<unsigned>(blocks < most ? blocks : most), 32 * kWarps, 0, stream>>>(p);
+}
 template <typename T>
-void launch_route(const agb::RouteParams& p, cudaStream_t stream) {
-  constexpr int kWarps = 4;
-  const unsigned grid = static_cast<unsigned>((p.tokens + kWarps - 1) / kWarps);
-  if (p.per_lane <= 1) agb::route_topk_kernel<T, 1><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else if (p.per_lane <= 2) agb::route_topk_kernel<T, 2><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else if (p.per_lane <= 4) agb::route_topk_kernel<T, 4><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else if (p.per_lane <= 8) agb::route_topk_kernel<T, 8><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else if (p.per_lane <= 16) agb::route_topk_kernel<T, 16><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else agb::route_topk_kernel<T, 32><<<grid, 32 * kWarps, 0, stream>>>(p);
+void launch_route(const agb::RouteParams& p, int sms, cudaStream_t stream) {
+  if (p.per_lane <= 1) launch_route_as<T, 1>(p, sms, stream);
+  else if (p.per_lane <= 2) launch_route_as<T, 2>(p, sms, stream);
+  else if (p.per_lane <= 4) launch_route_as<T, 4>(p, sms, stream);
+  else if (p.per_lane <= 8) launch_route_as<T, 8>(p, sms, stream);
+  else if (p.per_lane <= 16) launch_route_as<T, 16>(p, sms, stream);
+  else launch_route_as<T, 32>(p, sms, stream);
 }
 
 // Pairs per block: 4096 keep one block for a decode batch, and no more than 128 blocks, because every block sums the
@@ -679,6 +772,7 @@ int ag_route_topk(const ag_route_desc_t* r) {
   p.top_groups = r->top_groups;
   p.group_size = size;
   p.lanes_per_group = lanes;
+  while ((1 << p.lane_shift) < lanes) ++p.lane_shift;
   // a power of two of slots where that fills the lanes exactly (vector loads), else as few as hold the group
   p.per_lane = per;
   p.sigmoid = r->scoring == AG_SCORE_SIGMOID;
@@ -687,10 +781,12 @@ int ag_route_topk(const ag_route_desc_t* r) {
   p.scale = r->scale;
   const bool pow2 = (per & (per - 1)) == 0;
   p.vector_rows = pow2 && size == per * lanes && per * size_of(r->dtype) >= 16 && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
+  int sms = 0;
+  if (int rc = agb_device_sm_count(&sms)) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(r->stream);
-  if (r->dtype == AG_T_BF16) launch_route<__nv_bfloat16>(p, stream);
-  else if (r->dtype == AG_T_FP16) launch_route<__half>(p, stream);
-  else launch_route<float>(p, stream);
+  if (r->dtype == AG_T_BF16) launch_route<__nv_bfloat16>(p, sms, stream);
+  else if (r->dtype == AG_T_FP16) launch_route<__half>(p, sms, stream);
+  else launch_route<float>(p, sms, stream);
   return launch_check();
 }
 
