@@ -58,6 +58,12 @@ __device__ __forceinline__ double warp_sum_d(double v) {
 // A logit as the router counts it: NaN and -inf switch the expert off, +inf is the largest finite number.
 __device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINITY), FLT_MAX); }   // max(NaN, x) = x
 
+// Where a row's experts lie: every group on 1 << shift neighbouring lanes, per_lane consecutive experts on each.
+struct LaneMap {
+  int shift, per_lane;
+  int vector_rows, vector_bias;      // every lane's experts are full and 16-byte aligned in the logits / the bias
+};
+
 struct RouteParams {
   const void* logits;
   const float* bias;
@@ -65,19 +71,21 @@ struct RouteParams {
   long long* ids;
   float* weights;
   long long tokens, ld;
-  int experts, top_k, groups, top_groups, group_size, lanes_per_group, lane_shift, per_lane;   // lanes_per_group = 1 << lane_shift
-  int sigmoid, group_max, renormalize, vector_rows;
+  int experts, top_k, groups, top_groups, group_size;
+  int sigmoid, group_max, renormalize;
+  LaneMap warp;       // one row on the 32 lanes of a warp
+  LaneMap part;       // route_top8_kernel: one row on row_lanes lanes
+  int row_lanes, index_bits;
   float scale;
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-// One warp per token, persistent over tokens with the next row's load under way. The experts of a group lie on
-// `lanes_per_group` (a power of two) neighbouring lanes, `per_lane` consecutive ones each, so the lane order is the expert
-// order, a group's two best scores are a short shuffle reduction, and "lowest index among equals" is "lowest lane, then lowest
-// slot". Each lane sorts its experts once (lists of 8, as 32-bit keys that carry the slot in their lowest bits); the k best are
-// then taken off the heads of the lists, one warp-wide integer maximum and one predicated shift each: about 17 instructions
-// per expert where searching the lane's slots again took 60. With 256 experts the kernel executes some 500 instructions per
-// KB of logits and is bound by their issue, not by memory (65536 tokens: see the figures at launch_route).
+// Two kernels. route_topk_kernel (top_k above 8): one warp per token, persistent over tokens with the next row's load under
+// way. The lane order is the expert order, a group's two best scores are a short shuffle reduction, and "lowest index among
+// equals" is "lowest lane, then lowest slot". Each lane sorts its experts once (lists of 8, as 32-bit keys that carry the slot in
+// their lowest bits); the k best are then taken off the heads of the lists, one warp-wide integer maximum and one predicated
+// shift each. route_top8_kernel, below, has several tokens per warp. Both are bound by the instructions they issue, not by
+// memory (figures at launch_route).
 //
 // Order. Keys are scores in fp32, cut off at the slot bits; `tol` bounds what they are off by. A token with two neighbours in
 // the order, or two groups at the border, closer than that -- one in a few hundred -- is decided once more in 64 bits
@@ -85,17 +93,17 @@ struct RouteParams {
 // the formulas whatever the last bits of the exponentials are.
 struct Slots {
   int first, count;      // this lane holds the experts first .. first + count - 1
-  __device__ __forceinline__ Slots(const RouteParams& p, int lane) {
-    const int g = lane >> p.lane_shift, in = (lane & (p.lanes_per_group - 1)) * p.per_lane;
+  __device__ __forceinline__ Slots(const RouteParams& p, const LaneMap& map, int lane) {
+    const int g = lane >> map.shift, in = (lane & ((1 << map.shift) - 1)) * map.per_lane;
     first = g * p.group_size + in;
-    count = g < p.groups ? max(0, min(p.per_lane, p.group_size - in)) : 0;
+    count = g < p.groups ? max(0, min(map.per_lane, p.group_size - in)) : 0;
   }
 };
 
 // The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left).
 template <typename T, int VPL>
 __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
-  const Slots at(p, lane);
+  const Slots at(p, p.warp, lane);
   double c[VPL];
   double mx = -INFINITY;
 #pragma unroll
@@ -126,16 +134,16 @@ __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int 
       a2 = fmax(a2, fmin(a1, c[j]));
       a1 = fmax(a1, c[j]);
     }
-    for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+    for (int o = 1; o < (1 << p.warp.shift); o <<= 1) {
       const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
       a2 = fmax(fmax(a2, b2), fmin(a1, b1));
       a1 = fmax(a1, b1);
     }
     const double mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
-    const int g = lane >> p.lane_shift;
+    const int g = lane >> p.warp.shift;
     int rank = 0;
     for (int o = 0; o < p.groups; ++o) {
-      const double other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
+      const double other = __shfl_sync(kAll, mine, o << p.warp.shift);
       rank += other > mine || (other == mine && o < g);
     }
     if (rank >= p.top_groups) {
@@ -172,12 +180,12 @@ __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int 
   return chosen;
 }
 
-// Slots of one lane from memory. `vector_rows`: every lane's slots are full and 16-byte aligned.
+// Slots of one lane from a row of logits or the bias. `vector`: every lane's slots are full and 16-byte aligned.
 template <typename T, int VPL>
-__device__ __forceinline__ void load_slots(const RouteParams& p, const T* row, const Slots& at, float (&l)[VPL]) {
+__device__ __forceinline__ void load_slots(bool vector, const T* row, const Slots& at, float (&l)[VPL]) {
   constexpr int kBytes = VPL * static_cast<int>(sizeof(T));
   if constexpr (kBytes >= 16) {
-    if (p.vector_rows) {
+    if (vector) {
 #pragma unroll
       for (int q = 0; q < kBytes / 16; ++q) {
         uint4 v = make_uint4(0, 0, 0, 0);
@@ -241,15 +249,12 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
   const long long used = p.rows_used != nullptr ? *p.rows_used : p.tokens;
   const bool scored = p.bias != nullptr || p.groups > 1;      // the order needs the scores, not just the logits
-  const Slots at(p, lane);
+  const Slots at(p, p.warp, lane);
   float bias[VPL];
-  if (p.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) bias[j] = j < at.count ? clean(__ldg(p.bias + at.first + j)) : -INFINITY;
-  }
+  if (p.bias != nullptr) load_slots<float, VPL>(p.warp.vector_bias, p.bias, at, bias);
   long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   float next[VPL];
-  if (token < min(used, p.tokens)) load_slots<T, VPL>(p, static_cast<const T*>(p.logits) + token * p.ld, at, next);
+  if (token < min(used, p.tokens)) load_slots<T, VPL>(p.warp.vector_rows, static_cast<const T*>(p.logits) + token * p.ld, at, next);
 
   for (; token < p.tokens; token += warps) {
     long long* ids = p.ids + token * p.top_k;
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
     float c[VPL];      // what the experts are ordered by; -inf = off
 #pragma unroll
     for (int j = 0; j < VPL; ++j) c[j] = next[j];
-    if (token + warps < min(used, p.tokens)) load_slots<T, VPL>(p, row + warps * p.ld, at, next);
+    if (token + warps < min(used, p.tokens)) load_slots<T, VPL>(p.warp.vector_rows, row + warps * p.ld, at, next);
 
     float row_max = 0.f, sum = 0.f;
     if (!p.sigmoid && (scored || !p.renormalize)) {
@@ -307,16 +312,16 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
           a2 = fmaxf(a2, fminf(a1, s[j]));
           a1 = fmaxf(a1, s[j]);
         }
-        for (int o = 1; o < p.lanes_per_group; o <<= 1) {
+        for (int o = 1; o < (1 << p.warp.shift); o <<= 1) {
           const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
           a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
           a1 = fmaxf(a1, b1);
         }
         const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
-        const int g = lane >> p.lane_shift;
+        const int g = lane >> p.warp.shift;
         int rank = 0;
         for (int o = 0; o < p.groups; ++o) {
-          const float other = __shfl_sync(kAll, mine, o * p.lanes_per_group);
+          const float other = __shfl_sync(kAll, mine, o << p.warp.shift);
           rank += other > mine || (other == mine && o < g);
         }
         const bool kept = rank < p.top_groups, real = g < p.groups;
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
       }
     }
     auto expert_of = [&](int32_t key, int owner) {
-      const int g = owner >> p.lane_shift, in = (owner & (p.lanes_per_group - 1)) * p.per_lane;
+      const int g = owner >> p.warp.shift, in = (owner & ((1 << p.warp.shift) - 1)) * p.warp.per_lane;
       return key <= kOffKeys ? -1 : g * p.group_size + in + kSlotMask - (key & kSlotMask);
     };
     int chosen = expert_of(my_key, my_lane);
@@ -423,6 +428,259 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
       ids[lane] = chosen;
       weights[lane] = w * p.scale;
     }
+  }
+}
+
+// top_k up to 8: a row on `row_lanes` lanes, 32 / row_lanes rows per warp, so that what is done once per row -- ranking the groups,
+// joining the lanes' lists, the weights -- is done for several rows at once. Keys carry the expert's index in their lowest bits.
+// A lane sorts its experts in lists of 8 and merges them into its 8 best; the lanes' lists are merged by xor-shuffles (the
+// larger of a[i] and b[7 - i] are the 8 best of both, in bitonic order), after which every lane of the row has the answer
+// without a serial step per expert. The best key that a merge leaves out is kept: it says whether the eighth is clear of the rest.
+// Experts too close for their keys (the index takes 8 of 24 bits with 256 experts, so one token in twenty) are put in order by
+// their exact values, one per lane; only where the border itself is unclear does route_exact decide the row.
+__device__ __forceinline__ void bitonic8(int32_t (&a)[8]) {
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i & d) == 0) order(a[i], a[i + d]);
+  }
+}
+// a = the 8 largest of a and b (both sorted), sorted; `left` = the largest of those left out and what it was.
+__device__ __forceinline__ void merge8(int32_t (&a)[8], const int32_t (&b)[8], int32_t& left) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    left = max(left, min(a[i], b[7 - i]));
+    a[i] = max(a[i], b[7 - i]);
+  }
+  bitonic8(a);
+}
+
+// Experts first + 8 q .. of a lane, -inf past its last one.
+// RAW: without clean(), where the caller looks at all eight itself.
+template <typename T, bool RAW = false>
+__device__ __forceinline__ void load8(bool vector, const T* row, const Slots& at, int q, float (&l)[8]) {
+  const T* src = row + at.first + 8 * q;
+  if (vector && at.count > 0) {
+    constexpr int kWords = static_cast<int>(sizeof(T)) / 2;      // 16-byte words
+    uint4 u[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l[j] = RAW ? to_float(reinterpret_cast<const T*>(u)[j]) : clean(to_float(reinterpret_cast<const T*>(u)[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l[j] = 8 * q + j >= at.count ? -INFINITY : RAW ? to_float(src[j]) : clean(to_float(src[j]));
+  }
+}
+
+// Rolled over a lane's pieces of 8 experts: straight-line code for 32 of them did not fit the instruction cache. EXACT: slots per
+// lane that route_exact holds.
+template <typename T, int EXACT>
+__global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(const RouteParams p) {
+  const int lane = threadIdx.x & 31, width = p.row_lanes, in_row = lane & (width - 1), row0 = lane & ~(width - 1);
+  const int rows_per_warp = 32 / width;
+  const long long token0 = (static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * rows_per_warp;
+  if (token0 >= p.tokens) return;
+  const long long token = token0 + lane / width;
+  const bool exists = token < p.tokens, live = exists && (p.rows_used == nullptr || token < *p.rows_used);
+  const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+  auto row_max_of = [&](float v) {
+    for (int o = width >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+    return v;
+  };
+  auto row_sum_of = [&](float v) {
+    for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    return v;
+  };
+  const bool scored = p.bias != nullptr || p.groups > 1, softmax_all = !p.sigmoid && (scored || !p.renormalize);
+  Slots at(p, p.part, in_row);
+  if (!live) at.count = 0;
+  const int pieces = (p.part.per_lane + 7) >> 3;
+  float row_max = 0.f, sum = 0.f, inv = 0.f;
+  if (softmax_all) {      // two more walks over the row, out of L1 after the first
+    float mx = -INFINITY, l[8];
+    for (int q = 0; q < pieces; ++q) {
+      load8(p.part.vector_rows, row, at, q, l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, l[j]);
+    }
+    row_max = row_max_of(mx);
+    for (int q = 0; q < pieces; ++q) {
+      load8(p.part.vector_rows, row, at, q, l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += l[j] > -INFINITY ? __expf(l[j] - row_max) : 0.f;
+    }
+    sum = row_sum_of(sum);
+    inv = 1.f / sum;
+  }
+  const float tol = !scored ? 0.f : p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;      // as in route_topk_kernel
+
+  // the 8 best keys of this lane, the best one left out, and the two largest scores
+  const int32_t index_mask = (1 << p.index_bits) - 1;
+  int32_t top[8], left = INT32_MIN;
+  float a1 = -INFINITY, a2 = -INFINITY;
+  float c[8];
+  load8<T, true>(p.part.vector_rows, row, at, 0, c);
+#pragma unroll 1
+  for (int q = 0; q < pieces; ++q) {
+    float s[8], next[8];
+    if (q + 1 < pieces) load8<T, true>(p.part.vector_rows, row, at, q + 1, next);
+    // NaN, infinities and missing experts are rare: one look at the sum spares the common piece two operations per expert
+    float size = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) size += fabsf(c[j]);
+    const bool special = !(size < INFINITY);
+    if (special) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = clean(c[j]);
+    }
+    if (scored) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[j] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[j])) : __expf(c[j] - row_max) * inv;
+      }
+      if (p.bias != nullptr) {
+        float b[8];
+        load8(p.part.vector_bias, p.bias, at, q, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += b[j];      // a bias of -inf switches the expert off by itself
+      }
+      if (special) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+      }
+      if (p.groups > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          a2 = fmaxf(a2, fminf(a1, s[j]));
+          a1 = fmaxf(a1, s[j]);
+        }
+      }
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = s[j];
+      }
+    }
+    int32_t list[8];
+    const int32_t index0 = index_mask - (at.first + 8 * q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) list[j] = (key_of(c[j]) & ~index_mask) | ((index0 - j) & index_mask);
+    sort_list<8>(list);
+    if (q == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = list[j];
+    } else {
+      merge8(top, list, left);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = next[j];
+  }
+
+  bool unsure = false;
+  if (p.groups > 1) {
+    for (int o = 1; o < (1 << p.part.shift); o <<= 1) {
+      const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+      a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
+      a1 = fmaxf(a1, b1);
+    }
+    const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
+    const int g = in_row >> p.part.shift;
+    int rank = 0;
+    for (int o = 0; o < p.groups; ++o) {
+      const float other = __shfl_sync(kAll, mine, row0 + (o << p.part.shift));
+      rank += other > mine || (other == mine && o < g);
+    }
+    const bool kept = rank < p.top_groups, real = g < p.groups;
+    // the weakest group kept against the strongest one left out
+    const float low = -row_max_of(real && kept ? -mine : -INFINITY), high = row_max_of(real && !kept ? mine : -INFINITY);
+    if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
+    if (!kept) {
+      left = INT32_MIN;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top[j] = INT32_MIN;
+    }
+  }
+  // the 8 best keys of the row, on every lane of it
+  for (int o = 1; o < width; o <<= 1) {
+    int32_t other[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(kAll, top[j], o);
+    left = max(left, __shfl_xor_sync(kAll, left, o));
+    merge8(top, other, left);
+  }
+  // lane i of the row has the i-th best
+  int32_t key = kOffKeys;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) key = in_row == j ? top[j] : key;
+  auto expert_of = [&](int32_t k) { return k <= kOffKeys ? -1 : index_mask - (k & index_mask); };
+  int chosen = expert_of(key);
+
+  if (p.bias != nullptr || sizeof(T) == 4) {      // keys of 16-bit logits are exact: 13 bits above the index at least
+    int32_t next = __shfl_down_sync(kAll, key, 1);
+    if (in_row == 7) next = left;
+    const float v = value_of(key & ~index_mask), u = value_of(next & ~index_mask), off = p.bias != nullptr ? tol : 0.f;
+    const float cut = __int2float_rn(index_mask + 1) * 0x1p-23f + 0x1p-22f;
+    const bool close = in_row < 8 && key > kOffKeys && next > kOffKeys && !(v - u > 2.f * off + cut * (fabsf(v) + fabsf(u)));
+    const unsigned all_close = __ballot_sync(kAll, close);
+    if (all_close != 0u) {
+      const unsigned mine = (all_close >> row0) & 0xffu;
+      // what was left out may belong among the first top_k only if nothing separates it from them
+      const unsigned chain = 0xffu & ~((1u << (p.top_k - 1)) - 1u);
+      unsure = unsure || (mine & chain) == chain;
+      // a softmax score with a bias needs its sum in 64 bits too
+      if (mine != 0u && p.bias != nullptr && !p.sigmoid) unsure = true;
+      double d = -INFINITY;
+      if (mine != 0u && chosen >= 0) {
+        const float l = clean(to_float(row[chosen]));
+        d = p.bias == nullptr ? static_cast<double>(l) : 1 / (1 + exp(-static_cast<double>(l))) + static_cast<double>(clean(p.bias[chosen]));
+      }
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double e = __shfl_sync(kAll, d, row0 + j);
+        const int ej = __shfl_sync(kAll, chosen, row0 + j);
+        rank += e > d || (e == d && ej < chosen);
+      }
+      int sorted = -1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int rj = __shfl_sync(kAll, rank, row0 + j), ej = __shfl_sync(kAll, chosen, row0 + j);
+        if (ej >= 0 && rj == in_row) sorted = ej;
+      }
+      if (mine != 0u) chosen = sorted;
+    }
+  }
+  unsigned exact = __ballot_sync(kAll, unsure && live && in_row == 0);
+  while (exact != 0u) {
+    const int first = __ffs(exact) - 1;
+    exact &= exact - 1;
+    const int e = route_exact<T, EXACT>(p, static_cast<const T*>(p.logits) + (token0 + first / width) * p.ld, lane);
+    const int mine = __shfl_sync(kAll, e, in_row);
+    if (row0 == first) chosen = mine;
+  }
+  if (in_row >= p.top_k) chosen = -1;
+
+  const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
+  float w = 0.f;
+  if (p.renormalize) {      // as in route_topk_kernel
+    float best = row_max_of(l);
+    if (p.sigmoid) {
+      best = fminf(best, 0.f);
+      const float t = __expf(-fabsf(l));
+      w = __fdividef(l >= 0.f ? 1.f : __expf(l - best), 1.f + t);
+    } else {
+      w = __expf(l - best);
+    }
+    if (chosen < 0) w = 0.f;
+    const float total = row_sum_of(w);
+    w = chosen >= 0 ? __fdividef(w, total) : 0.f;
+  } else if (chosen >= 0) {
+    w = __fdividef(p.sigmoid ? 1.f : __expf(l - row_max), p.sigmoid ? 1.f + __expf(-l) : sum);
+  }
+  if (exists && in_row < p.top_k) {
+    p.ids[token * p.top_k + in_row] = chosen;
+    p.weights[token * p.top_k + in_row] = w * p.scale;
   }
 }
 
@@ -716,14 +974,43 @@ void launch_route_as(const agb::RouteParams& p, int sms, cudaStream_t stream) {
   const long long blocks = (p.tokens + kWarps - 1) / kWarps, most = static_cast<long long>(sms) * kBlocksPerSm;
   agb::route_topk_kernel<T, VPL><<<static_cast<unsigned>(blocks < most ? blocks : most), 32 * kWarps, 0, stream>>>(p);
 }
+template <typename T, int EXACT>
+void launch_top8_as(const agb::RouteParams& p, cudaStream_t stream) {
+  const long long rows = 4 * (32 / p.row_lanes);
+  agb::route_top8_kernel<T, EXACT><<<static_cast<unsigned>((p.tokens + rows - 1) / rows), 128, 0, stream>>>(p);
+}
 template <typename T>
 void launch_route(const agb::RouteParams& p, int sms, cudaStream_t stream) {
-  if (p.per_lane <= 1) launch_route_as<T, 1>(p, sms, stream);
-  else if (p.per_lane <= 2) launch_route_as<T, 2>(p, sms, stream);
-  else if (p.per_lane <= 4) launch_route_as<T, 4>(p, sms, stream);
-  else if (p.per_lane <= 8) launch_route_as<T, 8>(p, sms, stream);
-  else if (p.per_lane <= 16) launch_route_as<T, 16>(p, sms, stream);
-  else launch_route_as<T, 32>(p, sms, stream);
+  if (p.top_k <= 8) {
+    if (p.warp.per_lane <= 8) launch_top8_as<T, 8>(p, stream);
+    else if (p.warp.per_lane <= 16) launch_top8_as<T, 16>(p, stream);
+    else launch_top8_as<T, 32>(p, stream);
+  } else if (p.warp.per_lane <= 8) {
+    launch_route_as<T, 8>(p, sms, stream);
+  } else if (p.warp.per_lane <= 16) {
+    launch_route_as<T, 16>(p, sms, stream);
+  } else {
+    launch_route_as<T, 32>(p, sms, stream);
+  }
+}
+
+// The map of a row onto `lanes` lanes; per_lane is above 32 where they are too few.
+agb::LaneMap lane_map(const ag_route_desc_t* r, int lanes) {
+  agb::LaneMap m{};
+  int across = lanes;
+  while (across * r->groups > lanes) across >>= 1;
+  if (across == 0) {
+    m.per_lane = agb::kRouteMaxPerLane + 1;
+    return m;
+  }
+  while ((1 << m.shift) < across) ++m.shift;
+  const int size = r->experts / r->groups;
+  m.per_lane = (size + across - 1) / across;
+  // vector loads want lanes full of slots, 8, 16 or 32 of them
+  const bool full = (m.per_lane & (m.per_lane - 1)) == 0 && m.per_lane >= 8 && size == m.per_lane * across;
+  m.vector_rows = full && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
+  m.vector_bias = full && aligned_to(r->bias, 16);
+  return m;
 }
 
 // Pairs per block: 4096 keep one block for a decode batch, and no more than 128 blocks, because every block sums the
@@ -748,10 +1035,8 @@ int ag_route_topk(const ag_route_desc_t* r) {
   const int size = r->experts / r->groups;
   if (r->top_k > agb::kRouteMaxTopK || r->top_k > r->top_groups * size)
     return agb_fail(AG_E_INVALID, "top_k must be at most 32 and at most the experts of top_groups groups");
-  int lanes = 32;
-  while (lanes * r->groups > 32) lanes >>= 1;
-  const int per = (size + lanes - 1) / lanes;
-  if (per > agb::kRouteMaxPerLane) return agb_fail(AG_E_INVALID, "too many experts (at most 32 per lane: 1024 in one group, 1024 / groups rounded to a power of two in each of several)");
+  const agb::LaneMap warp = lane_map(r, 32);
+  if (warp.per_lane > agb::kRouteMaxPerLane) return agb_fail(AG_E_INVALID, "too many experts (at most 32 per lane: 1024 in one group, 1024 / groups rounded to a power of two in each of several)");
   if (!aligned_to(r->logits, size_of(r->dtype)) || !aligned_to(r->bias, 4) || !aligned_to(r->rows_used, 4) || !aligned_to(r->ids, 8) ||
       !aligned_to(r->weights, 4))
     return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
@@ -771,18 +1056,17 @@ int ag_route_topk(const ag_route_desc_t* r) {
   p.groups = r->groups;
   p.top_groups = r->top_groups;
   p.group_size = size;
-  p.lanes_per_group = lanes;
-  while ((1 << p.lane_shift) < lanes) ++p.lane_shift;
-  // a power of two of slots where that fills the lanes exactly (vector loads), else as few as hold the group
-  p.per_lane = per;
+  p.warp = warp;
   p.sigmoid = r->scoring == AG_SCORE_SIGMOID;
   p.group_max = r->group_max != 0;
   p.renormalize = r->renormalize != 0;
   p.scale = r->scale;
-  const bool pow2 = (per & (per - 1)) == 0;
-  p.vector_rows = pow2 && size == per * lanes && per * size_of(r->dtype) >= 16 && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
   int sms = 0;
   if (int rc = agb_device_sm_count(&sms)) return rc;
+  // Few tokens: a row on a whole warp, for the shorter way through it. Many: as few lanes as hold it, for the fewer instructions.
+  p.row_lanes = r->tokens <= 4 * sms ? 32 : 8;
+  while ((p.part = lane_map(r, p.row_lanes)).per_lane > agb::kRouteMaxPerLane) p.row_lanes *= 2;
+  while ((1 << p.index_bits) < r->experts) ++p.index_bits;
   cudaStream_t stream = static_cast<cudaStream_t>(r->stream);
   if (r->dtype == AG_T_BF16) launch_route<__nv_bfloat16>(p, sms, stream);
   else if (r->dtype == AG_T_FP16) launch_route<__half>(p, sms, stream);
