@@ -53,23 +53,33 @@ __device__ __forceinline__ void store_from_float(void* p, long long i, int type,
   else static_cast<float*>(p)[i] = v;
 }
 
+__device__ __forceinline__ float reciprocal(float x) {      // 1 ulp, 0 for infinity
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Phi(z) = erfc(-z / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (absolute error of erfc 1.5e-7): five products and one exponential
-// without a branch. The exact functions of the library cost an epilogue twice its time and change no 16-bit result.
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float x = fabsf(z) * 0.70710678f;
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  float c = fmaf(1.061405429f, t, -1.453152027f);
-  c = fmaf(c, t, 1.421413741f);
-  c = fmaf(c, t, -0.284496736f);
-  c = fmaf(c, t, 0.254829592f);
-  const float tail = 0.5f * c * t * __expf(-x * x);
+// without a branch. The exact functions of the library cost an epilogue twice its time and change no 16-bit result. `bell` is
+// exp(-z^2 / 2), which the density needs too.
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  bell = __expf(-0.5f * z * z);
+  const float t = reciprocal(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+  float c = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  c = fmaf(c, t, 0.5f * 1.421413741f);
+  c = fmaf(c, t, 0.5f * -0.284496736f);
+  c = fmaf(c, t, 0.5f * 0.254829592f);
+  const float tail = c * t * bell;
   return z < 0.f ? tail : 1.f - tail;
 }
 
 __device__ __forceinline__ float activate(float z, int act) {
   if (act == ACT_RELU) return z < 0.f ? 0.f : z;                       // NaN stays NaN
-  if (act == ACT_GELU) return z * normal_cdf(z);
-  if (act == ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
+  if (act == ACT_GELU) {
+    float bell;
+    return z * normal_cdf(z, bell);
+  }
+  if (act == ACT_SILU) return z * reciprocal(1.f + __expf(-z));
   return z;
 }
 

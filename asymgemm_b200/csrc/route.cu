@@ -696,11 +696,11 @@ struct RouteGradParams {
   const long long* ids;
   void* dlogits;
   long long tokens, ld;
-  int experts, top_k, sigmoid, renormalize, vector_rows;
+  int experts, top_k, sigmoid, renormalize;
   float scale;
 };
 
-template <typename T>
+template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGradParams p) {
   const long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -752,14 +752,14 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
     dot = warp_sum_f(s * g);
     v = s * g;
   }
-  constexpr int V = 16 / static_cast<int>(sizeof(T));
-  const int step = p.vector_rows ? V : 1;
-  for (int e0 = lane * step; e0 - lane * step < p.experts; e0 += 32 * step) {   // every lane of the warp takes every round
+  constexpr int V = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 1;      // elements a lane writes at once
+  for (int first = 0; first < p.experts; first += 32 * V) {            // every lane of the warp takes every round
+    const int e0 = first + lane * V;
     float a[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       a[i] = 0.f;
-      if (dense && i < step && e0 + i < p.experts) {
+      if (dense && e0 + i < p.experts) {
         const float x = clean(to_float(row[e0 + i]));
         if (x > -INFINITY) a[i] = -expf(x - row_max) * inv * dot;
       }
@@ -768,18 +768,16 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
       const int at = __shfl_sync(kAll, id, t) - e0;
       const float add = __shfl_sync(kAll, v, t);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (at == i) a[i] += add;
+      for (int i = 0; i < V; ++i) a[i] += at == i ? add : 0.f;
     }
-    if (p.vector_rows) {
-      if (e0 < p.experts) {
-        uint4 o;
-        T* t = reinterpret_cast<T*>(&o);
+    if (e0 >= p.experts) continue;
+    if constexpr (VECTOR) {
+      uint4 o;
+      T* t = reinterpret_cast<T*>(&o);
 #pragma unroll
-        for (int i = 0; i < V; ++i) t[i] = from_float<T>(a[i]);
-        *reinterpret_cast<uint4*>(out + e0) = o;
-      }
-    } else if (e0 < p.experts) {
+      for (int i = 0; i < V; ++i) t[i] = from_float<T>(a[i]);
+      *reinterpret_cast<uint4*>(out + e0) = o;
+    } else {
       out[e0] = from_float<T>(a[0]);
     }
   }
@@ -848,11 +846,26 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
   const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
   const long long share = p.run / kLayoutWarps;            // a multiple of 32
   const long long from = begin + warp * share, to = min(from + share, end);
-  for (long long i0 = from; i0 < to; i0 += 32) {
-    const int e = i0 + lane < to ? pair_expert(p, i0 + lane, true) : -1;
-    const unsigned same = __match_any_sync(kAll, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] += __popc(same);
-    __syncwarp();
+  // the warp's pairs, kept in registers 4 x 32 at a time so that their loads are under way together (a run of 4096 pairs per
+  // block is just that; a longer one is read again below)
+  constexpr int kAhead = 4;
+  int mine_e[kAhead];
+  auto load_pairs = [&](long long i0, bool report) {
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const long long i = i0 + 32 * q + lane;
+      mine_e[q] = i < to ? pair_expert(p, i, report) : -1;
+    }
+  };
+  for (long long i0 = from; i0 < to; i0 += 32 * kAhead) {
+    load_pairs(i0, true);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const int e = mine_e[q];
+      const unsigned same = __match_any_sync(kAll, e);
+      if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] += __popc(same);
+      __syncwarp();
+    }
   }
   if (!ONE) {
     // all blocks' counts, `parts` threads per expert; integer sums, so their order does not matter
@@ -860,6 +873,7 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
     for (int i = threadIdx.x; i < parts * E; i += kLayoutThreads) {
       const int e = i % E;
       int all = 0, before = 0;
+#pragma unroll 8
       for (int b = i / E; b < static_cast<int>(gridDim.x); b += parts) {
         const int v = __ldg(p.block_counts + static_cast<long long>(b) * E + e);
         all += v;
@@ -922,39 +936,34 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
     }
     __syncthreads();
   }
-  for (long long i0 = from; i0 < to; i0 += 32) {
-    const long long i = i0 + lane;
-    const int e = i < to ? pair_expert(p, i, false) : -1;
-    const unsigned same = __match_any_sync(kAll, e);
-    int base = 0;
-    if (e >= 0) base = mine[warp * E + e];
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] = base + __popc(same);
-    __syncwarp();
-    if (i < to) {
-      const int within = base + __popc(same & ((1u << lane) - 1u));
-      const bool placed = e >= 0 && (p.max_rows == 0 || within < p.max_rows);
-      const long long row = placed ? static_cast<long long>(start[e]) + within : -1;
-      p.pair_row[i] = row;
-      if (placed) p.row_token[row] = i / p.top_k;
+  for (long long i0 = from; i0 < to; i0 += 32 * kAhead) {
+    if (to - from > 32 * kAhead) load_pairs(i0, false);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      const long long i = i0 + 32 * q + lane;
+      const int e = mine_e[q];
+      const unsigned same = __match_any_sync(kAll, e);
+      int base = 0;
+      if (e >= 0) base = mine[warp * E + e];
+      __syncwarp();
+      if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] = base + __popc(same);
+      __syncwarp();
+      if (i < to) {
+        const int within = base + __popc(same & ((1u << lane) - 1u));
+        const bool placed = e >= 0 && (p.max_rows == 0 || within < p.max_rows);
+        const long long row = placed ? static_cast<long long>(start[e]) + within : -1;
+        p.pair_row[i] = row;
+        if (placed) p.row_token[row] = i / p.top_k;
+      }
     }
   }
-  // rows that no pair has: -1, each block a run of them
-  const long long rows_run = (p.rows + gridDim.x - 1) / gridDim.x;
-  const long long r_end = min((blockIdx.x + 1) * rows_run, p.rows);
-  for (long long r = blockIdx.x * rows_run + threadIdx.x; r < r_end; r += kLayoutThreads) {
-    if (r >= start[E]) {
-      p.row_token[r] = -1;
-      continue;
-    }
-    int lo = 0, hi = E;                // the last segment that starts at or before r (empty ones share their start with the next)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (start[mid] <= r) lo = mid;
-      else hi = mid;
-    }
-    if (r - start[lo] >= total[lo]) p.row_token[r] = -1;
+  // rows that no pair has: the end of every expert's segment, a warp of the launch each, and what lies behind the last
+  for (int e = blockIdx.x * kLayoutWarps + warp; e < E; e += gridDim.x * kLayoutWarps) {
+    const int end_row = start[e + 1];
+    for (int r = start[e] + min(total[e], end_row - start[e]) + lane; r < end_row; r += 32) p.row_token[r] = -1;
   }
+  for (long long r = start[E] + static_cast<long long>(blockIdx.x) * kLayoutThreads + threadIdx.x; r < p.rows; r += static_cast<long long>(gridDim.x) * kLayoutThreads)
+    p.row_token[r] = -1;
 }
 
 }  // namespace agb
@@ -1011,6 +1020,13 @@ agb::LaneMap lane_map(const ag_route_desc_t* r, int lanes) {
   m.vector_rows = full && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
   m.vector_bias = full && aligned_to(r->bias, 16);
   return m;
+}
+
+template <typename T>
+void launch_route_backward(const agb::RouteGradParams& p, bool vector, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>((p.tokens + 3) / 4);
+  if (vector) agb::route_topk_backward_kernel<T, true><<<grid, 128, 0, stream>>>(p);
+  else agb::route_topk_backward_kernel<T, false><<<grid, 128, 0, stream>>>(p);
 }
 
 // Pairs per block: 4096 keep one block for a decode batch, and no more than 128 blocks, because every block sums the
@@ -1097,12 +1113,11 @@ int ag_route_topk_backward(const void* logits, int32_t dtype, int64_t tokens, in
   p.sigmoid = scoring == AG_SCORE_SIGMOID;
   p.renormalize = renormalize != 0;
   p.scale = scale;
-  p.vector_rows = static_cast<int64_t>(experts) * size % 16 == 0 && aligned_to(dlogits, 16);
-  const unsigned grid = static_cast<unsigned>((tokens + 3) / 4);
+  const bool vector = static_cast<int64_t>(experts) * size % 16 == 0 && aligned_to(dlogits, 16);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == AG_T_BF16) agb::route_topk_backward_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else if (dtype == AG_T_FP16) agb::route_topk_backward_kernel<__half><<<grid, 128, 0, s>>>(p);
-  else agb::route_topk_backward_kernel<float><<<grid, 128, 0, s>>>(p);
+  if (dtype == AG_T_BF16) launch_route_backward<__nv_bfloat16>(p, vector, s);
+  else if (dtype == AG_T_FP16) launch_route_backward<__half>(p, vector, s);
+  else launch_route_backward<float>(p, vector, s);
   return launch_check();
 }
 
