@@ -33,10 +33,10 @@ ALIGN = 128
 @dataclass
 class DispatchState:
     """Everything `combine` needs to send results back and undo the permutations of `dispatch`."""
-    order: torch.Tensor          # [T*k] positions of the (token, slot) pairs sorted by expert
+    order: Optional[torch.Tensor]  # [T*k] positions of the (token, slot) pairs sorted by expert
     send_splits: List[int]       # rows sent to each rank
     recv_splits: List[int]       # rows received from each rank
-    dest_rows: torch.Tensor      # [R] row of every received row in the padded contiguous layout
+    dest_rows: Optional[torch.Tensor]  # [R] row of every received row in the padded contiguous layout
     rows_per_expert: torch.Tensor  # [experts_per_rank] valid rows of every local expert (device tensor)
     padded_rows: int             # rows allocated for the contiguous layout (upper bound; every expert padded to 128)
     offsets: torch.Tensor        # int32 [2*experts_per_rank] (start, end) pairs; empty experts have start == end
@@ -44,6 +44,7 @@ class DispatchState:
     tokens: int
     top_k: int
     src_token: Optional[torch.Tensor] = None   # one rank only: rows were not gathered yet; received row i is token src_token[i]
+    tables: Optional[moe_ops.RouteLayout] = None   # one rank on a GPU: the layout's tables in place of order, dest_rows, src_token
 
 
 class EPDispatcher:
@@ -134,9 +135,16 @@ class EPDispatcher:
         rows [T, H] (any dtype; FP8 rows travel as bytes), extras: more per-token tensors [T, *] sent alongside (scales).
         Returns (state, recv_rows [R, H], recv_extras). With one rank nothing leaves the device and the host never
         waits; with several ranks the split sizes of the exchange are read back once, on a side stream, so the host
-        does not wait for GEMMs still running on the compute stream.
+        does not wait for GEMMs still running on the compute stream. On one GPU the layout comes from `moe_ops.route_layout`
+        (one or two kernels; pairs with id -1, as `moe_ops.route_topk` marks padding tokens, get no row).
         """
         tokens, top_k = topk_ids.shape
+        if self.world == 1 and topk_ids.is_cuda and self.num_experts <= moe_ops.MAX_LAYOUT_EXPERTS and topk_ids.dtype in (torch.int64, torch.int32):
+            tables = moe_ops.route_layout(topk_ids.contiguous(), self.num_experts, ALIGN)
+            splits = [tokens * top_k]
+            state = DispatchState(None, splits, splits, None, tables.rows_per_expert, tables.row_token.numel(), tables.offsets, tables.experts,
+                                  tokens, top_k, tables=tables)
+            return state, rows, tuple(extras)
         if self.world == 1:
             order, send_counts, recv_counts = self.plan(topk_ids)
             send_splits = recv_splits = [tokens * top_k]
@@ -281,6 +289,10 @@ class EPDispatcher:
     def combine(self, expert_out: torch.Tensor, state: DispatchState, topk_weights: torch.Tensor, mark=None) -> torch.Tensor:
         """expert_out [padded_rows, H] (contiguous layout) -> y [T, H] = sum_k w[t, k] * out(t, k), in fp32, as expert_out.dtype.
         `mark(name)`, if given, is called between the return exchange and the weighted sum (phase timing)."""
+        if state.tables is not None:
+            if mark is not None:
+                mark("return")
+            return moe_ops.combine_topk(expert_out, state.tables.pair_row, topk_weights, state.tokens, state.top_k)
         # inverse of the sort: pair p (token p // k, slot p % k) was sent as sorted row inv[p]
         inv = torch.empty_like(state.order)
         inv[state.order] = torch.arange(state.order.numel(), device=state.order.device)
@@ -299,7 +311,10 @@ class EPDispatcher:
 
 
 def to_contiguous_layout(recv: torch.Tensor, state: DispatchState) -> torch.Tensor:
-    """Scatter received rows into the zero-padded contiguous layout the grouped GEMM consumes."""
+    """Scatter received rows into the zero-padded contiguous layout the grouped GEMM consumes (one rank on a GPU: gather them,
+    which writes every row, padding included, once)."""
+    if state.tables is not None:
+        return moe_ops.move_rows(recv.contiguous(), state.padded_rows, src_rows=state.tables.row_token)
     return moe_ops.move_rows(recv.contiguous(), state.padded_rows, src_rows=state.src_token, dst_rows=state.dest_rows, zero=True)
 
 

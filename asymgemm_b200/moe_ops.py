@@ -86,7 +86,8 @@ def _row_bytes(t: torch.Tensor) -> int:
 
 def move_rows(src: torch.Tensor, out_rows: int, src_rows: Optional[torch.Tensor] = None, dst_rows: Optional[torch.Tensor] = None,
               count: Optional[int] = None, zero: bool = False) -> torch.Tensor:
-    """out[dst_rows[i] or i] = src[src_rows[i] or i] for i < count. `out` has `out_rows` rows of src's row shape and dtype."""
+    """out[dst_rows[i] or i] = src[src_rows[i] or i] for i < count. `out` has `out_rows` rows of src's row shape and dtype.
+    A negative src_rows[i] writes a row of zeros, a negative dst_rows[i] writes nothing."""
     count = int(count if count is not None else (src_rows.numel() if src_rows is not None else
                                                  (dst_rows.numel() if dst_rows is not None else src.shape[0])))
     out = (torch.zeros if zero else torch.empty)((out_rows,) + tuple(src.shape[1:]), dtype=src.dtype, device=src.device)
@@ -101,9 +102,14 @@ def move_rows(src: torch.Tensor, out_rows: int, src_rows: Optional[torch.Tensor]
         return out
     s = src.view(torch.uint8) if src.dtype == torch.float8_e4m3fn else src
     o = out.view(torch.uint8) if out.dtype == torch.float8_e4m3fn else out
-    picked = s.index_select(0, src_rows) if src_rows is not None else s[:count]
+    if src_rows is not None:
+        picked = s.index_select(0, src_rows.clamp(min=0))
+        picked.masked_fill_((src_rows < 0).view((-1,) + (1,) * (s.dim() - 1)), 0)
+    else:
+        picked = s[:count]
     if dst_rows is not None:
-        o.index_copy_(0, dst_rows, picked)
+        keep = dst_rows >= 0
+        o.index_copy_(0, dst_rows[keep], picked[keep])
     else:
         o[:count] = picked
     return out
@@ -149,7 +155,9 @@ def _combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, 
             _lib.check(_lib.load().ag_combine_topk_f32(rows.data_ptr(), pos.data_ptr(), w.data_ptr(), y.data_ptr(), tokens, top_k, cols,
                                                        _stream(rows)))
         return y
-    picked = (rows.index_select(0, pos) if pos is not None else rows[: tokens * top_k]).view(tokens, top_k, cols).float()
+    picked = (rows.index_select(0, pos.clamp(min=0)) if pos is not None else rows[: tokens * top_k]).view(tokens, top_k, cols).float()
+    if pos is not None:
+        picked = torch.where((pos < 0).view(tokens, top_k, 1), picked.new_zeros(()), picked)
     return (picked * weights.unsqueeze(-1).float()).sum(dim=1).to(rows.dtype)
 
 
@@ -185,6 +193,7 @@ class _CombineTopK(torch.autograd.Function):
 
 
 # --------------------------------------------------------------------------------------------- routing
+MAX_LAYOUT_EXPERTS = 1024      # experts that route_layout builds tables for
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"top2": False, "max": True}
 

@@ -456,3 +456,21 @@ def test_route_layout_and_combine_together_in_a_captured_graph():
     # every token's rows are its own x: the combine gives x back where the weights sum to 1
     y, xs = out[2][:280].double(), x[:280].double()
     assert bool(((y - xs).abs() <= xs.abs() * (2 ** -8 + 16 * 2 ** -22)).all()) and float(out[2][280:].abs().max()) == 0
+
+
+@pytest.mark.parametrize("tokens,experts,k,cols,dtype", [(37, 8, 3, 64, torch.bfloat16), (1, 256, 8, 32, torch.bfloat16), (700, 60, 4, 20, torch.float32)])
+def test_dispatcher_on_one_gpu_lays_rows_out_as_on_the_cpu(tokens, experts, k, cols, dtype):
+    from asymgemm_b200.ep import EPDispatcher, to_contiguous_layout
+    disp = EPDispatcher(experts)
+    ids, x = make_ids(tokens, experts, k, 90), randn(tokens, cols, seed=91, dtype=dtype)
+    w = torch.rand((tokens, k), generator=torch.Generator().manual_seed(92))
+    cpu, rows_cpu, _ = disp.dispatch(x.cpu(), ids)
+    gpu, rows_gpu, _ = disp.dispatch(x, ids.to(DEV))
+    a_cpu, a_gpu = to_contiguous_layout(rows_cpu, cpu), to_contiguous_layout(rows_gpu, gpu)
+    assert torch.equal(a_gpu.cpu(), a_cpu) and gpu.padded_rows == cpu.padded_rows
+    assert torch.equal(gpu.offsets.cpu(), cpu.offsets) and torch.equal(gpu.experts.cpu(), cpu.experts)
+    assert torch.equal(gpu.rows_per_expert.cpu(), cpu.rows_per_expert)
+    y_cpu, y_gpu = disp.combine(a_cpu, cpu, w), disp.combine(a_gpu, gpu, w.to(DEV))
+    # k products and additions in fp32, then one rounding to bf16 (the CPU rounds to the rows' type)
+    size = (a_cpu.double().abs().max() * w.double().sum(1).max()).item()
+    assert bool(((y_gpu.cpu().double() - y_cpu.double()).abs() <= 2 ** -7 * y_cpu.double().abs() + size * 2 * k * 2 ** -24).all())
