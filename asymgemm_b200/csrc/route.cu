@@ -44,15 +44,10 @@ __device__ __forceinline__ float warp_sum_f(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   return v;
 }
-__device__ __forceinline__ double warp_max_d(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, o));
-  return v;
-}
-__device__ __forceinline__ double warp_sum_d(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-  return v;
+__device__ __forceinline__ float reciprocal(float x) {      // 1 ulp, 0 for infinity
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // A logit as the router counts it: NaN and -inf switch the expert off, +inf is the largest finite number.
@@ -61,7 +56,8 @@ __device__ __forceinline__ float clean(float l) { return fminf(fmaxf(l, -INFINIT
 // Where a row's experts lie: every group on 1 << shift neighbouring lanes, per_lane consecutive experts on each.
 struct LaneMap {
   int shift, per_lane;
-  int vector_rows, vector_bias;      // every lane's experts are full and 16-byte aligned in the logits / the bias
+  int vector_rows, vector_bias;      // every lane's experts are full and 16-byte aligned in the logits / the bias:
+  int lane_shift;                    // then per_lane = 1 << lane_shift
 };
 
 struct RouteParams {
@@ -80,8 +76,7 @@ struct RouteParams {
 };
 
 // ------------------------------------------------------------------------------------------------ forward
-// Two kernels. route_topk_kernel (top_k above 8): one warp per token, persistent over tokens with the next row's load under
-// way. The lane order is the expert order, a group's two best scores are a short shuffle reduction, and "lowest index among
+// Two kernels. route_topk_kernel (top_k above 8): one warp per token (route_row). The lane order is the expert order, a group's two best scores are a short shuffle reduction, and "lowest index among
 // equals" is "lowest lane, then lowest slot". Each lane sorts its experts once (lists of 8, as 32-bit keys that carry the slot in
 // their lowest bits); the k best are then taken off the heads of the lists, one warp-wide integer maximum and one predicated
 // shift each. route_top8_kernel, below, has several tokens per warp. Both are bound by the instructions they issue, not by
@@ -100,40 +95,41 @@ struct Slots {
   }
 };
 
-// The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left).
-template <typename T, int VPL>
+// The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left). Every loop is rolled: the code runs for
+// a handful of rows per SM, so what it costs is fetching its instructions (unrolled, the 65536 x 256 case took 58 us instead of
+// 47).
+template <typename T>
 __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
   const Slots at(p, p.warp, lane);
-  double c[VPL];
-  double mx = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    c[j] = j < at.count ? static_cast<double>(clean(to_float(row[at.first + j]))) : -INFINITY;
-    mx = fmax(mx, c[j]);
+  double c[kRouteMaxPerLane], mx = -INFINITY, sum = 0;
+  auto logit = [&](int j) { return static_cast<double>(clean(to_float(row[at.first + j]))); };
+  auto everyone = [&](double v, auto join) {
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(kAll, v, o));
+    return v;
+  };
+  auto larger = [](double a, double b) { return fmax(a, b); };
+#pragma unroll 1
+  for (int j = 0; j < at.count; ++j) mx = fmax(mx, logit(j));
+  if (!p.sigmoid) mx = everyone(mx, larger);
+#pragma unroll 1
+  for (int j = 0; j < at.count; ++j) {
+    const double l = logit(j), e = exp(p.sigmoid ? -l : l - mx);
+    c[j] = l == -INFINITY ? -INFINITY : p.sigmoid ? 1 / (1 + e) : e;
+    if (l > -INFINITY) sum += e;
   }
-  mx = warp_max_d(mx);
-  double sum = 0;
-  if (!p.sigmoid) {
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? exp(c[j] - mx) : 0;
-    sum = warp_sum_d(sum);
+  if (!p.sigmoid) sum = everyone(sum, [](double a, double b) { return a + b; });
+  double a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll 1
+  for (int j = 0; j < at.count; ++j) {
+    if (!p.sigmoid) c[j] /= sum;
+    if (p.bias != nullptr) c[j] += static_cast<double>(clean(p.bias[at.first + j]));      // -inf on either side: off
+    a2 = fmax(a2, fmin(a1, c[j]));
+    a1 = fmax(a1, c[j]);
   }
-#pragma unroll
-  for (int j = 0; j < VPL; ++j) {
-    if (c[j] == -INFINITY) continue;
-    c[j] = p.sigmoid ? 1 / (1 + exp(-c[j])) : exp(c[j] - mx) / sum;
-    if (p.bias != nullptr) {
-      const float b = clean(p.bias[at.first + j]);
-      c[j] = b == -INFINITY ? -INFINITY : c[j] + static_cast<double>(b);
-    }
-  }
+  bool kept = true;
   if (p.groups > 1) {
-    double a1 = -INFINITY, a2 = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      a2 = fmax(a2, fmin(a1, c[j]));
-      a1 = fmax(a1, c[j]);
-    }
+#pragma unroll 1
     for (int o = 1; o < (1 << p.warp.shift); o <<= 1) {
       const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
       a2 = fmax(fmax(a2, b2), fmin(a1, b1));
@@ -142,39 +138,32 @@ __device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int 
     const double mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
     const int g = lane >> p.warp.shift;
     int rank = 0;
+#pragma unroll 1
     for (int o = 0; o < p.groups; ++o) {
       const double other = __shfl_sync(kAll, mine, o << p.warp.shift);
       rank += other > mine || (other == mine && o < g);
     }
-    if (rank >= p.top_groups) {
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) c[j] = -INFINITY;
-    }
+    kept = rank < p.top_groups;
   }
   // without a bias the scores rise with the logits: among the groups kept, the logits themselves are the exact order
-  if (p.bias == nullptr) {
-#pragma unroll
-    for (int j = 0; j < VPL; ++j)
-      if (c[j] > -INFINITY) c[j] = static_cast<double>(clean(to_float(row[at.first + j])));
-  }
+#pragma unroll 1
+  for (int j = 0; j < at.count; ++j) c[j] = !kept ? -INFINITY : p.bias == nullptr && c[j] > -INFINITY ? logit(j) : c[j];
   int chosen = -1;
+#pragma unroll 1
   for (int i = 0; i < p.top_k; ++i) {
     double m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) m = fmax(m, c[j]);
-    const double best = warp_max_d(m);
-    if (best == -INFINITY) break;
-    const int w = __ffs(__ballot_sync(kAll, m == best)) - 1;
-    int e = -1;
-    if (lane == w) {
-#pragma unroll
-      for (int j = 0; j < VPL; ++j)
-        if (e < 0 && c[j] == best) {
-          e = at.first + j;
-          c[j] = -INFINITY;
-        }
+    int slot = 0;
+#pragma unroll 1
+    for (int j = 0; j < at.count; ++j) {
+      if (c[j] > m) {
+        m = c[j];
+        slot = j;
+      }
     }
-    e = __shfl_sync(kAll, e, w);
+    const double best = everyone(m, larger);
+    if (best == -INFINITY) break;
+    const int w = __ffs(__ballot_sync(kAll, m == best)) - 1, e = __shfl_sync(kAll, at.first + slot, w);
+    if (lane == w) c[slot] = -INFINITY;
     if (lane == i) chosen = e;
   }
   return chosen;
@@ -241,22 +230,158 @@ __device__ __forceinline__ void sort_list(int32_t (&s)[N]) {
   }
 }
 
+// The selection for one row on a whole warp: returns the expert chosen i-th on lane i (-1: none left), and, where a softmax over
+// the whole row was taken, its maximum and sum.
 template <typename T, int VPL>
-__global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
+__device__ __forceinline__ int route_row(const RouteParams& p, const T* row, int lane, float& row_max, float& sum) {
   constexpr int kLen = VPL < 8 ? VPL : 8, kLists = VPL / kLen;
   constexpr int32_t kSlotMask = VPL - 1;      // key bits that hold VPL - 1 - slot
+  const bool scored = p.bias != nullptr || p.groups > 1;      // the order needs the scores, not just the logits
+  const Slots at(p, p.warp, lane);
+  float c[VPL];      // what the experts are ordered by; -inf = off
+  load_slots<T, VPL>(p.warp.vector_rows, row, at, c);
+  row_max = sum = 0.f;
+  if (!p.sigmoid && (scored || !p.renormalize)) {
+    float mx = c[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
+    row_max = warp_max_f(mx);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? __expf(c[j] - row_max) : 0.f;
+    sum = warp_sum_f(sum);
+  }
+  bool unsure = false;
+  float tol = 0.f;
+  if (scored) {
+    float s[VPL];
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      s[j] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[j])) : __expf(c[j] - row_max) * inv;
+    }
+    bool any_off = false;      // rare, so the common row has no select per expert
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) any_off = any_off || c[j] == -INFINITY;
+    // Error of a score. Sigmoid: s (1 - s) |l| 2^-23 from the exponential's argument, a few roundings of a number <= 1.
+    // Softmax, of numbers <= 1 / sum: d e^-d 2^-23 for l = max - d, and up to 37 additions in the sum.
+    tol = p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;
+    if (p.bias != nullptr) {
+      float bias[VPL];
+      load_slots<float, VPL>(p.warp.vector_bias, p.bias, at, bias);
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) s[j] += bias[j];      // a bias of -inf switches the expert off by itself
+    }
+    if (any_off) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+    }
+    if (p.groups > 1) {
+      float a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        a2 = fmaxf(a2, fminf(a1, s[j]));
+        a1 = fmaxf(a1, s[j]);
+      }
+      for (int o = 1; o < (1 << p.warp.shift); o <<= 1) {
+        const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+        a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
+        a1 = fmaxf(a1, b1);
+      }
+      const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
+      const int g = lane >> p.warp.shift;
+      int rank = 0;
+      for (int o = 0; o < p.groups; ++o) {
+        const float other = __shfl_sync(kAll, mine, o << p.warp.shift);
+        rank += other > mine || (other == mine && o < g);
+      }
+      const bool kept = rank < p.top_groups, real = g < p.groups;
+      // the weakest group kept against the strongest one left out
+      const float low = -warp_max_f(real && kept ? -mine : -INFINITY), high = warp_max_f(real && !kept ? mine : -INFINITY);
+      if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
+      if (!kept) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) s[j] = c[j] = -INFINITY;
+      }
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) c[j] = s[j];
+    }
+  }
+
+  int32_t list[kLists][kLen];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) list[j / kLen][j % kLen] = (key_of(c[j]) & ~kSlotMask) | (VPL - 1 - j);
+#pragma unroll
+  for (int q = 0; q < kLists; ++q) sort_list<kLen>(list[q]);
+
+  int32_t my_key = kOffKeys;      // lane i: the key and lane of the expert taken i-th
+  int my_lane = 0;
+  auto head = [&] {
+    int32_t h = list[0][0];
+#pragma unroll
+    for (int q = 1; q < kLists; ++q) h = max(h, list[q][0]);
+    return h;
+  };
+  // The best head by value, of equal ones the lowest lane's (the slot bits order experts within a lane only).
+  auto take_best = [&](int32_t h, int& w) {
+    const int32_t value = __reduce_max_sync(kAll, h & ~kSlotMask);
+    w = __ffs(__ballot_sync(kAll, (h & ~kSlotMask) == value)) - 1;
+    return __shfl_sync(kAll, h, w);
+  };
+  for (int i = 0; i < p.top_k; ++i) {
+    int w;
+    const int32_t best = take_best(head(), w);
+    if (best <= kOffKeys) break;
+#pragma unroll
+    for (int q = 0; q < kLists; ++q) {
+      const bool pop = lane == w && list[q][0] == best;
+#pragma unroll
+      for (int j = 0; j + 1 < kLen; ++j) list[q][j] = pop ? list[q][j + 1] : list[q][j];
+      list[q][kLen - 1] = pop ? INT32_MIN : list[q][kLen - 1];
+    }
+    if (lane == i) {
+      my_key = best;
+      my_lane = w;
+    }
+  }
+  auto expert_of = [&](int32_t key, int owner) {
+    const int g = owner >> p.warp.shift, in = (owner & ((1 << p.warp.shift) - 1)) * p.warp.per_lane;
+    return key <= kOffKeys ? -1 : g * p.group_size + in + kSlotMask - (key & kSlotMask);
+  };
+  int chosen = expert_of(my_key, my_lane);
+  {
+    // each expert taken against the next in the order: lane top_k - 1's next is the first one left out
+    int out_lane;
+    const int32_t out = take_best(head(), out_lane);
+    int32_t next_key = __shfl_down_sync(kAll, my_key, 1);
+    int next_e = __shfl_down_sync(kAll, chosen, 1);
+    if (lane == p.top_k - 1) {
+      next_key = out;
+      next_e = expert_of(out, out_lane);
+    }
+    const float v = value_of(my_key & ~kSlotMask), u = value_of(next_key & ~kSlotMask);
+    constexpr float kCut = VPL * 0x1p-23f + 0x1p-22f;      // the slot bits cut off, half a step of the sum with the bias
+    const float off = p.bias != nullptr ? tol : 0.f;
+    bool close = lane < p.top_k && my_key > kOffKeys && next_key > kOffKeys && !(v - u > 2.f * off + kCut * (fabsf(v) + fabsf(u)));
+    if (__any_sync(kAll, close)) {
+      if (close) {
+        close = clean(to_float(row[chosen])) != clean(to_float(row[next_e])) ||
+                (p.bias != nullptr && clean(p.bias[chosen]) != clean(p.bias[next_e]));
+      }
+      unsure = unsure || __any_sync(kAll, close);
+    }
+  }
+  if (unsure) chosen = route_exact<T>(p, row, lane);
+  return lane < p.top_k ? chosen : -1;
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
   const long long used = p.rows_used != nullptr ? *p.rows_used : p.tokens;
-  const bool scored = p.bias != nullptr || p.groups > 1;      // the order needs the scores, not just the logits
-  const Slots at(p, p.warp, lane);
-  float bias[VPL];
-  if (p.bias != nullptr) load_slots<float, VPL>(p.warp.vector_bias, p.bias, at, bias);
-  long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  float next[VPL];
-  if (token < min(used, p.tokens)) load_slots<T, VPL>(p.warp.vector_rows, static_cast<const T*>(p.logits) + token * p.ld, at, next);
-
-  for (; token < p.tokens; token += warps) {
+  for (long long token = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); token < p.tokens; token += warps) {
     long long* ids = p.ids + token * p.top_k;
     float* weights = p.weights + token * p.top_k;
     if (token >= used) {      // a padding token is routed nowhere
@@ -267,143 +392,8 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
       continue;
     }
     const T* row = static_cast<const T*>(p.logits) + token * p.ld;
-    float c[VPL];      // what the experts are ordered by; -inf = off
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) c[j] = next[j];
-    if (token + warps < min(used, p.tokens)) load_slots<T, VPL>(p.warp.vector_rows, row + warps * p.ld, at, next);
-
-    float row_max = 0.f, sum = 0.f;
-    if (!p.sigmoid && (scored || !p.renormalize)) {
-      float mx = c[0];
-#pragma unroll
-      for (int j = 1; j < VPL; ++j) mx = fmaxf(mx, c[j]);
-      row_max = warp_max_f(mx);
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) sum += c[j] > -INFINITY ? __expf(c[j] - row_max) : 0.f;
-      sum = warp_sum_f(sum);
-    }
-    bool unsure = false;
-    float tol = 0.f;
-    if (scored) {
-      float s[VPL];
-      const float inv = 1.f / sum;
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        s[j] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[j])) : __expf(c[j] - row_max) * inv;
-      }
-      bool any_off = false;      // rare, so the common row has no select per expert
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) any_off = any_off || c[j] == -INFINITY;
-      // Error of a score. Sigmoid: s (1 - s) |l| 2^-23 from the exponential's argument, a few roundings of a number <= 1.
-      // Softmax, of numbers <= 1 / sum: d e^-d 2^-23 for l = max - d, and up to 37 additions in the sum.
-      tol = p.sigmoid ? 0x1p-20f : 0x1p-18f * inv;
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] += bias[j];      // a bias of -inf switches the expert off by itself
-      }
-      if (any_off) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
-      }
-      if (p.groups > 1) {
-        float a1 = -INFINITY, a2 = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) {
-          a2 = fmaxf(a2, fminf(a1, s[j]));
-          a1 = fmaxf(a1, s[j]);
-        }
-        for (int o = 1; o < (1 << p.warp.shift); o <<= 1) {
-          const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
-          a2 = fmaxf(fmaxf(a2, b2), fminf(a1, b1));
-          a1 = fmaxf(a1, b1);
-        }
-        const float mine = p.group_max || a2 == -INFINITY ? a1 : a1 + a2;
-        const int g = lane >> p.warp.shift;
-        int rank = 0;
-        for (int o = 0; o < p.groups; ++o) {
-          const float other = __shfl_sync(kAll, mine, o << p.warp.shift);
-          rank += other > mine || (other == mine && o < g);
-        }
-        const bool kept = rank < p.top_groups, real = g < p.groups;
-        // the weakest group kept against the strongest one left out
-        const float low = -warp_max_f(real && kept ? -mine : -INFINITY), high = warp_max_f(real && !kept ? mine : -INFINITY);
-        if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
-        if (!kept) {
-#pragma unroll
-          for (int j = 0; j < VPL; ++j) s[j] = c[j] = -INFINITY;
-        }
-      }
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < VPL; ++j) c[j] = s[j];
-      }
-    }
-
-    int32_t list[kLists][kLen];
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) list[j / kLen][j % kLen] = (key_of(c[j]) & ~kSlotMask) | (VPL - 1 - j);
-#pragma unroll
-    for (int q = 0; q < kLists; ++q) sort_list<kLen>(list[q]);
-
-    int32_t my_key = kOffKeys;      // lane i: the key and lane of the expert taken i-th
-    int my_lane = 0;
-    auto head = [&] {
-      int32_t h = list[0][0];
-#pragma unroll
-      for (int q = 1; q < kLists; ++q) h = max(h, list[q][0]);
-      return h;
-    };
-    // The best head by value, of equal ones the lowest lane's (the slot bits order experts within a lane only).
-    auto take_best = [&](int32_t h, int& w) {
-      const int32_t value = __reduce_max_sync(kAll, h & ~kSlotMask);
-      w = __ffs(__ballot_sync(kAll, (h & ~kSlotMask) == value)) - 1;
-      return __shfl_sync(kAll, h, w);
-    };
-    for (int i = 0; i < p.top_k; ++i) {
-      int w;
-      const int32_t best = take_best(head(), w);
-      if (best <= kOffKeys) break;
-#pragma unroll
-      for (int q = 0; q < kLists; ++q) {
-        const bool pop = lane == w && list[q][0] == best;
-#pragma unroll
-        for (int j = 0; j + 1 < kLen; ++j) list[q][j] = pop ? list[q][j + 1] : list[q][j];
-        list[q][kLen - 1] = pop ? INT32_MIN : list[q][kLen - 1];
-      }
-      if (lane == i) {
-        my_key = best;
-        my_lane = w;
-      }
-    }
-    auto expert_of = [&](int32_t key, int owner) {
-      const int g = owner >> p.warp.shift, in = (owner & ((1 << p.warp.shift) - 1)) * p.warp.per_lane;
-      return key <= kOffKeys ? -1 : g * p.group_size + in + kSlotMask - (key & kSlotMask);
-    };
-    int chosen = expert_of(my_key, my_lane);
-    {
-      // each expert taken against the next in the order: lane top_k - 1's next is the first one left out
-      int out_lane;
-      const int32_t out = take_best(head(), out_lane);
-      int32_t next_key = __shfl_down_sync(kAll, my_key, 1);
-      int next_e = __shfl_down_sync(kAll, chosen, 1);
-      if (lane == p.top_k - 1) {
-        next_key = out;
-        next_e = expert_of(out, out_lane);
-      }
-      const float v = value_of(my_key & ~kSlotMask), u = value_of(next_key & ~kSlotMask);
-      constexpr float kCut = VPL * 0x1p-23f + 0x1p-22f;      // the slot bits cut off, half a step of the sum with the bias
-      const float off = p.bias != nullptr ? tol : 0.f;
-      bool close = lane < p.top_k && my_key > kOffKeys && next_key > kOffKeys && !(v - u > 2.f * off + kCut * (fabsf(v) + fabsf(u)));
-      if (__any_sync(kAll, close)) {
-        if (close) {
-          close = clean(to_float(row[chosen])) != clean(to_float(row[next_e])) ||
-                  (p.bias != nullptr && clean(p.bias[chosen]) != clean(p.bias[next_e]));
-        }
-        unsure = unsure || __any_sync(kAll, close);
-      }
-    }
-    if (unsure) chosen = route_exact<T, VPL>(p, row, lane);
-
+    float row_max, sum;
+    const int chosen = route_row<T, VPL>(p, row, lane, row_max, sum);
     // Weights, lane i for the expert chosen i-th. Sums over at most 32 chosen experts, in fp32.
     const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
     float w = 0.f;
@@ -456,28 +446,29 @@ __device__ __forceinline__ void merge8(int32_t (&a)[8], const int32_t (&b)[8], i
   bitonic8(a);
 }
 
-// Experts first + 8 q .. of a lane, -inf past its last one.
-// RAW: without clean(), where the caller looks at all eight itself.
+// Experts 8 q .. of a lane whose `count` experts start at `mine`, -inf past the last one. RAW: without clean(), where the caller
+// looks at all eight itself.
 template <typename T, bool RAW = false>
-__device__ __forceinline__ void load8(bool vector, const T* row, const Slots& at, int q, float (&l)[8]) {
-  const T* src = row + at.first + 8 * q;
-  if (vector && at.count > 0) {
+__device__ __forceinline__ void load8(bool vector, const T* mine, int count, int q, float (&l)[8]) {
+  const T* src = mine + 8 * q;
+  if (vector && count > 0) {
     constexpr int kWords = static_cast<int>(sizeof(T)) / 2;      // 16-byte words
     uint4 u[kWords];
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    for (int i = 0; i < kWords; ++i) u[i] = reinterpret_cast<const uint4*>(src)[i];
 #pragma unroll
     for (int j = 0; j < 8; ++j) l[j] = RAW ? to_float(reinterpret_cast<const T*>(u)[j]) : clean(to_float(reinterpret_cast<const T*>(u)[j]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l[j] = 8 * q + j >= at.count ? -INFINITY : RAW ? to_float(src[j]) : clean(to_float(src[j]));
+    for (int j = 0; j < 8; ++j) l[j] = 8 * q + j >= count ? -INFINITY : RAW ? to_float(src[j]) : clean(to_float(src[j]));
   }
 }
 
-// Rolled over a lane's pieces of 8 experts: straight-line code for 32 of them did not fit the instruction cache. EXACT: slots per
-// lane that route_exact holds.
-template <typename T, int EXACT>
-__global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(const RouteParams p) {
+// Rolled over a lane's pieces of 8 experts: straight-line code for 32 of them did not fit the instruction cache. STAGED: the warp's rows come through shared memory by 16-byte asynchronous copies, each lane's
+// experts 16 bytes further apart there; read straight from memory, lanes 64 bytes or more apart take a cache line each for 16
+// bytes (65536 x 256 fp32: 57 us so, with that and the 64-bit comparison of every close pair).
+template <typename T, bool STAGED>
+__global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31, width = p.row_lanes, in_row = lane & (width - 1), row0 = lane & ~(width - 1);
   const int rows_per_warp = 32 / width;
   const long long token0 = (static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * rows_per_warp;
@@ -485,6 +476,34 @@ __global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(con
   const long long token = token0 + lane / width;
   const bool exists = token < p.tokens, live = exists && (p.rows_used == nullptr || token < *p.rows_used);
   const T* row = static_cast<const T*>(p.logits) + token * p.ld;
+  Slots at(p, p.part, in_row);
+  if (!live) at.count = 0;
+  extern __shared__ uint4 route_smem[];
+  const int lane_bytes = p.part.per_lane * static_cast<int>(sizeof(T));      // STAGED: a multiple of 64
+  char* stage = reinterpret_cast<char*>(route_smem) + (threadIdx.x >> 5) * 32 * (lane_bytes + 16);
+  const T* mine = row + at.first;
+  if constexpr (STAGED) {
+    const int row_bytes = p.experts * static_cast<int>(sizeof(T));
+    const long long limit = p.rows_used == nullptr ? p.tokens : min(p.tokens, static_cast<long long>(*p.rows_used));
+    for (int r = 0; r < rows_per_warp && token0 + r < limit; ++r) {
+      const char* src = reinterpret_cast<const char*>(static_cast<const T*>(p.logits) + (token0 + r) * p.ld);
+      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(stage + r * width * (lane_bytes + 16)));
+      for (int byte = lane * 16; byte < row_bytes; byte += 512)      // 16 bytes of padding per lane before this one
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + byte + (byte / static_cast<int>(sizeof(T)) >> p.part.lane_shift) * 16), "l"(src + byte) : "memory");
+    }
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    mine = reinterpret_cast<const T*>(stage + lane * (lane_bytes + 16));
+  }
+  // logit of an expert of this lane's row
+  auto logit = [&](int e) {
+    if constexpr (STAGED) {
+      const int owner = e >> p.part.lane_shift;
+      return clean(to_float(reinterpret_cast<const T*>(stage + (row0 + owner) * (lane_bytes + 16))[e - (owner << p.part.lane_shift)]));
+    } else {
+      return clean(to_float(row[e]));
+    }
+  };
   auto row_max_of = [&](float v) {
     for (int o = width >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
     return v;
@@ -494,20 +513,18 @@ __global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(con
     return v;
   };
   const bool scored = p.bias != nullptr || p.groups > 1, softmax_all = !p.sigmoid && (scored || !p.renormalize);
-  Slots at(p, p.part, in_row);
-  if (!live) at.count = 0;
   const int pieces = (p.part.per_lane + 7) >> 3;
   float row_max = 0.f, sum = 0.f, inv = 0.f;
   if (softmax_all) {      // two more walks over the row, out of L1 after the first
     float mx = -INFINITY, l[8];
     for (int q = 0; q < pieces; ++q) {
-      load8(p.part.vector_rows, row, at, q, l);
+      load8(p.part.vector_rows, mine, at.count, q, l);
 #pragma unroll
       for (int j = 0; j < 8; ++j) mx = fmaxf(mx, l[j]);
     }
     row_max = row_max_of(mx);
     for (int q = 0; q < pieces; ++q) {
-      load8(p.part.vector_rows, row, at, q, l);
+      load8(p.part.vector_rows, mine, at.count, q, l);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += l[j] > -INFINITY ? __expf(l[j] - row_max) : 0.f;
     }
@@ -521,34 +538,44 @@ __global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(con
   int32_t top[8], left = INT32_MIN;
   float a1 = -INFINITY, a2 = -INFINITY;
   float c[8];
-  load8<T, true>(p.part.vector_rows, row, at, 0, c);
+  load8<T, true>(p.part.vector_rows, mine, at.count, 0, c);
 #pragma unroll 1
   for (int q = 0; q < pieces; ++q) {
     float s[8], next[8];
-    if (q + 1 < pieces) load8<T, true>(p.part.vector_rows, row, at, q + 1, next);
+    if (q + 1 < pieces) load8<T, true>(p.part.vector_rows, mine, at.count, q + 1, next);
     // NaN, infinities and missing experts are rare: one look at the sum spares the common piece two operations per expert
     float size = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) size += fabsf(c[j]);
+    float b[8];
+    if (p.bias != nullptr) {
+      load8<float, true>(p.part.vector_bias, p.bias + at.first, at.count, q, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) size += fabsf(b[j]);
+    }
     const bool special = !(size < INFINITY);
     if (special) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[j] = clean(c[j]);
     }
     if (scored) {
+      if (p.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        s[j] = p.sigmoid ? __fdividef(1.f, 1.f + __expf(-c[j])) : __expf(c[j] - row_max) * inv;
-      }
-      if (p.bias != nullptr) {
-        float b[8];
-        load8(p.part.vector_bias, p.bias, at, q, b);
+        for (int j = 0; j < 8; ++j) s[j] = reciprocal(1.f + __expf(-c[j]));
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] += b[j];      // a bias of -inf switches the expert off by itself
+        for (int j = 0; j < 8; ++j) s[j] = __expf(c[j] - row_max) * inv;
       }
       if (special) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+        for (int j = 0; j < 8; ++j) {
+          s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+          if (p.bias != nullptr) b[j] = clean(b[j]);
+        }
+      }
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += b[j];      // a bias of -inf switches the expert off by itself
       }
       if (p.groups > 1) {
 #pragma unroll
@@ -563,9 +590,15 @@ __global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(con
       }
     }
     int32_t list[8];
-    const int32_t index0 = index_mask - (at.first + 8 * q);
+    if (p.part.vector_rows) {      // the first expert is a multiple of 8: its index is or'ed in with the slot's
+      const int32_t index = (index_mask - 7) - (at.first + 8 * q);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) list[j] = (key_of(c[j]) & ~index_mask) | ((index0 - j) & index_mask);
+      for (int j = 0; j < 8; ++j) list[j] = ((key_of(c[j]) & ~index_mask) | index) | (7 - j);
+    } else {
+      const int32_t index0 = index_mask - (at.first + 8 * q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) list[j] = (key_of(c[j]) & ~index_mask) | ((index0 - j) & index_mask);
+    }
     sort_list<8>(list);
     if (q == 0) {
 #pragma unroll
@@ -624,44 +657,62 @@ __global__ void __launch_bounds__(128, EXACT <= 8 ? 8 : 4) route_top8_kernel(con
     const bool close = in_row < 8 && key > kOffKeys && next > kOffKeys && !(v - u > 2.f * off + cut * (fabsf(v) + fabsf(u)));
     const unsigned all_close = __ballot_sync(kAll, close);
     if (all_close != 0u) {
-      const unsigned mine = (all_close >> row0) & 0xffu;
+      const unsigned here = (all_close >> row0) & 0xffu;
       // what was left out may belong among the first top_k only if nothing separates it from them
       const unsigned chain = 0xffu & ~((1u << (p.top_k - 1)) - 1u);
-      unsure = unsure || (mine & chain) == chain;
-      // a softmax score with a bias needs its sum in 64 bits too
-      if (mine != 0u && p.bias != nullptr && !p.sigmoid) unsure = true;
-      double d = -INFINITY;
-      if (mine != 0u && chosen >= 0) {
-        const float l = clean(to_float(row[chosen]));
-        d = p.bias == nullptr ? static_cast<double>(l) : 1 / (1 + exp(-static_cast<double>(l))) + static_cast<double>(clean(p.bias[chosen]));
-      }
-      int rank = 0;
+      unsure = unsure || (here & chain) == chain;
+      // in order by the whole fp32 value, then, where even that is within its error of the next, by the exact one
+      const float l = chosen >= 0 ? logit(chosen) : -INFINITY, b = p.bias != nullptr && chosen >= 0 ? clean(p.bias[chosen]) : 0.f;
+      float f = l;
+      if (p.bias != nullptr && chosen >= 0) f = (p.sigmoid ? __fdividef(1.f, 1.f + __expf(-l)) : __expf(l - row_max) * inv) + b;
+      auto sort_by = [&](auto value) {
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const auto v = __shfl_sync(kAll, value, row0 + j);
+          const int e = __shfl_sync(kAll, chosen, row0 + j);
+          rank += v > value || (v == value && e < chosen);
+        }
+        int sorted = -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = __shfl_sync(kAll, rank, row0 + j), e = __shfl_sync(kAll, chosen, row0 + j);
+          if (e >= 0 && r == in_row) sorted = e;
+        }
+        return sorted;
+      };
+      // two with the same logit and bias are in the right order already, by index, and need no more
+      bool alike = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double e = __shfl_sync(kAll, d, row0 + j);
-        const int ej = __shfl_sync(kAll, chosen, row0 + j);
-        rank += e > d || (e == d && ej < chosen);
+        const float fj = __shfl_sync(kAll, f, row0 + j), lj = __shfl_sync(kAll, l, row0 + j), bj = __shfl_sync(kAll, b, row0 + j);
+        alike = alike || (in_row < 8 && chosen >= 0 && (lj != l || bj != b) && lj > -INFINITY && !(fabsf(fj - f) > 2.f * off + 0x1p-22f * (fabsf(fj) + fabsf(f))));
       }
-      int sorted = -1;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int rj = __shfl_sync(kAll, rank, row0 + j), ej = __shfl_sync(kAll, chosen, row0 + j);
-        if (ej >= 0 && rj == in_row) sorted = ej;
+      alike = alike && p.bias != nullptr;      // logits alone are exact
+      int sorted = sort_by(f);
+      const unsigned all_alike = __ballot_sync(kAll, alike);
+      if (all_alike != 0u) {
+        if (p.sigmoid) {
+          const double d = chosen >= 0 ? 1 / (1 + exp(-static_cast<double>(l))) + static_cast<double>(b) : -INFINITY;
+          sorted = sort_by(d);
+        } else if (((all_alike >> row0) & 0xffu) != 0u) {
+          unsure = true;      // a softmax score needs its sum in 64 bits too
+        }
       }
-      if (mine != 0u) chosen = sorted;
+      if (here != 0u) chosen = sorted;
     }
   }
   unsigned exact = __ballot_sync(kAll, unsure && live && in_row == 0);
   while (exact != 0u) {
     const int first = __ffs(exact) - 1;
     exact &= exact - 1;
-    const int e = route_exact<T, EXACT>(p, static_cast<const T*>(p.logits) + (token0 + first / width) * p.ld, lane);
-    const int mine = __shfl_sync(kAll, e, in_row);
-    if (row0 == first) chosen = mine;
+    const int e = route_exact<T>(p, static_cast<const T*>(p.logits) + (token0 + first / width) * p.ld, lane);
+    const int theirs = __shfl_sync(kAll, e, in_row);
+    if (row0 == first) chosen = theirs;
   }
   if (in_row >= p.top_k) chosen = -1;
 
-  const float l = chosen >= 0 ? clean(to_float(row[chosen])) : -INFINITY;
+  const float l = chosen >= 0 ? logit(chosen) : -INFINITY;
   float w = 0.f;
   if (p.renormalize) {      // as in route_topk_kernel
     float best = row_max_of(l);
@@ -983,17 +1034,20 @@ void launch_route_as(const agb::RouteParams& p, int sms, cudaStream_t stream) {
   const long long blocks = (p.tokens + kWarps - 1) / kWarps, most = static_cast<long long>(sms) * kBlocksPerSm;
   agb::route_topk_kernel<T, VPL><<<static_cast<unsigned>(blocks < most ? blocks : most), 32 * kWarps, 0, stream>>>(p);
 }
-template <typename T, int EXACT>
-void launch_top8_as(const agb::RouteParams& p, cudaStream_t stream) {
+template <typename T>
+void launch_top8(const agb::RouteParams& p, cudaStream_t stream) {
   const long long rows = 4 * (32 / p.row_lanes);
-  agb::route_top8_kernel<T, EXACT><<<static_cast<unsigned>((p.tokens + rows - 1) / rows), 128, 0, stream>>>(p);
+  const unsigned grid = static_cast<unsigned>((p.tokens + rows - 1) / rows);
+  const int lane_bytes = p.part.per_lane * static_cast<int>(sizeof(T));
+  if (p.part.vector_rows && lane_bytes >= 64)
+    agb::route_top8_kernel<T, true><<<grid, 128, 128 * (lane_bytes + 16), stream>>>(p);
+  else
+    agb::route_top8_kernel<T, false><<<grid, 128, 0, stream>>>(p);
 }
 template <typename T>
 void launch_route(const agb::RouteParams& p, int sms, cudaStream_t stream) {
   if (p.top_k <= 8) {
-    if (p.warp.per_lane <= 8) launch_top8_as<T, 8>(p, stream);
-    else if (p.warp.per_lane <= 16) launch_top8_as<T, 16>(p, stream);
-    else launch_top8_as<T, 32>(p, stream);
+    launch_top8<T>(p, stream);
   } else if (p.warp.per_lane <= 8) {
     launch_route_as<T, 8>(p, sms, stream);
   } else if (p.warp.per_lane <= 16) {
@@ -1017,6 +1071,7 @@ agb::LaneMap lane_map(const ag_route_desc_t* r, int lanes) {
   m.per_lane = (size + across - 1) / across;
   // vector loads want lanes full of slots, 8, 16 or 32 of them
   const bool full = (m.per_lane & (m.per_lane - 1)) == 0 && m.per_lane >= 8 && size == m.per_lane * across;
+  while (full && (1 << m.lane_shift) < m.per_lane) ++m.lane_shift;
   m.vector_rows = full && aligned_to(r->logits, 16) && r->ld * size_of(r->dtype) % 16 == 0;
   m.vector_bias = full && aligned_to(r->bias, 16);
   return m;
