@@ -82,7 +82,7 @@ def build_torch_ops(force: bool = False) -> Path:
             cmd += ["-isystem", inc]
         for lib in ce.library_paths():
             cmd += ["-L", lib]
-        cmd += ["-L", str(LIB_DIR), "-lasymgemm_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+        cmd += ["-L", str(LIB_DIR), "-lasymgemm_b200", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN"]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             last = f"{cxx}: building the torch extension failed:\n{res.stdout}\n{res.stderr}"

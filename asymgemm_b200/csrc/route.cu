@@ -868,6 +868,7 @@ __device__ __forceinline__ int pair_expert(const LayoutParams& p, long long i, b
 
 __global__ void __launch_bounds__(kLayoutThreads) layout_count_kernel(const LayoutParams p) {
   extern __shared__ int count[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the next kernel starts on its own pairs meanwhile
   for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) count[e] = 0;
   __syncthreads();
   const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
@@ -919,14 +920,15 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
     }
   }
   if (!ONE) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // the counts are complete
     // all blocks' counts, `parts` threads per expert; integer sums, so their order does not matter
     const int parts = max(1, kLayoutThreads / E);
     for (int i = threadIdx.x; i < parts * E; i += kLayoutThreads) {
       const int e = i % E;
       int all = 0, before = 0;
-#pragma unroll 8
+#pragma unroll 16
       for (int b = i / E; b < static_cast<int>(gridDim.x); b += parts) {
-        const int v = __ldg(p.block_counts + static_cast<long long>(b) * E + e);
+        const int v = __ldcg(p.block_counts + static_cast<long long>(b) * E + e);
         all += v;
         before += b < static_cast<int>(blockIdx.x) ? v : 0;
       }
@@ -1004,7 +1006,7 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
         const bool placed = e >= 0 && (p.max_rows == 0 || within < p.max_rows);
         const long long row = placed ? static_cast<long long>(start[e]) + within : -1;
         p.pair_row[i] = row;
-        if (placed) p.row_token[row] = i / p.top_k;
+        if (placed) p.row_token[row] = static_cast<unsigned>(i) / static_cast<unsigned>(p.top_k);      // pairs < 2^30
       }
     }
   }
@@ -1233,7 +1235,20 @@ int ag_route_layout(const ag_route_layout_desc_t* r) {
     if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   }
   if (blocks > 1) agb::layout_count_kernel<<<blocks, agb::kLayoutThreads, static_cast<size_t>(r->experts) * 4, stream>>>(p);
-  place<<<blocks, agb::kLayoutThreads, smem, stream>>>(p);
+  // Launched while the counting kernel runs: it counts its own pairs before it waits for the others' counts. It writes nothing
+  // but shared memory and the status word before that.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(agb::kLayoutThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, place, p);
+  if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   return launch_check();
 }
 

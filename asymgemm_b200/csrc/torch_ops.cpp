@@ -5,6 +5,7 @@
 // Python). No arithmetic happens here and the GEMM operator allocates nothing; the library below it has no torch
 // dependency.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -114,6 +115,11 @@ void m_grouped_gemm_nt(int64_t kind, int64_t layout, const at::Tensor& a, const 
 // These allocate their outputs (and what workspace they need) through torch on the current stream, so that a captured
 // graph owns them, and launch like the operator above.
 
+// Uninitialised tensors from the caching allocator on the current stream, without the dispatcher's way there.
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
 void check_ok(int rc) { TORCH_CHECK(rc == AG_OK, "asymgemm_b200: ", ag_last_error(), " (code ", rc, ")"); }
 
 int32_t type_code(at::ScalarType t, const char* name) {
@@ -149,8 +155,8 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits, int64_t 
   ag_route_desc_t d{};
   d.dtype = type_code(logits.scalar_type(), "logits");
   const c10::cuda::CUDAGuard guard(logits.device());
-  at::Tensor ids = at::empty({tokens, top_k}, logits.options().dtype(at::kLong));
-  at::Tensor weights = at::empty({tokens, top_k}, logits.options().dtype(at::kFloat));
+  at::Tensor ids = empty({tokens, top_k}, at::kLong, logits);
+  at::Tensor weights = empty({tokens, top_k}, at::kFloat, logits);
   d.logits = logits.data_ptr();
   d.ld = row_stride(logits);
   d.bias = static_cast<const float*>(ptr_of(bias));
@@ -180,7 +186,7 @@ at::Tensor route_topk_backward(const at::Tensor& dweights, const at::Tensor& ids
   check_same_device(dweights, "dweights", logits, at::kFloat, ids.numel());
   const int32_t type = type_code(logits.scalar_type(), "logits");
   const c10::cuda::CUDAGuard guard(logits.device());
-  at::Tensor dlogits = at::empty({logits.size(0), logits.size(1)}, logits.options());
+  at::Tensor dlogits = empty({logits.size(0), logits.size(1)}, logits.scalar_type(), logits);
   check_ok(ag_route_topk_backward(logits.data_ptr(), type, logits.size(0), row_stride(logits), static_cast<int32_t>(logits.size(1)),
                                   static_cast<const float*>(dweights.data_ptr()), static_cast<const int64_t*>(ids.data_ptr()),
                                   static_cast<int32_t>(ids.size(1)), static_cast<int32_t>(scoring), renormalize, static_cast<float>(scale),
@@ -202,7 +208,7 @@ void run_layout(ag_route_layout_desc_t& d, const at::Tensor& ids, int64_t expert
   const uint64_t need = ag_route_layout_workspace_bytes(ids.numel(), static_cast<int32_t>(experts));
   at::Tensor workspace;
   if (need > 0) {
-    workspace = at::empty({static_cast<int64_t>(need)}, ids.options().dtype(at::kByte));
+    workspace = empty({static_cast<int64_t>(need)}, at::kByte, ids);
     d.workspace = workspace.data_ptr();
     d.workspace_bytes = need;
   }
@@ -227,9 +233,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_lay
   const int64_t pairs = ids.numel();
   const int64_t rows = pairs > 0 ? (pairs + alignment - 1) / alignment * alignment + experts * alignment : 0;
   const c10::cuda::CUDAGuard guard(ids.device());
-  const auto i64 = ids.options().dtype(at::kLong), i32 = ids.options().dtype(at::kInt);
-  at::Tensor pair_row = at::empty({pairs}, i64), row_token = at::empty({rows}, i64), rows_per_expert = at::empty({experts}, i64);
-  at::Tensor offsets = at::empty({2 * experts}, i32), expert_list = at::empty({experts + 1}, i32);
+  at::Tensor pair_row = empty({pairs}, at::kLong, ids), row_token = empty({rows}, at::kLong, ids), rows_per_expert = empty({experts}, at::kLong, ids);
+  at::Tensor offsets = empty({2 * experts}, at::kInt, ids), expert_list = empty({experts + 1}, at::kInt, ids);
   ag_route_layout_desc_t d{};
   d.alignment = static_cast<int32_t>(alignment);
   d.rows_per_expert = static_cast<int64_t*>(rows_per_expert.data_ptr());
@@ -243,9 +248,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_layout_masked(const at::Ten
   check_layout_args(ids, experts, status);
   TORCH_CHECK(max_rows > 0 && max_rows < (int64_t{1} << 31) / experts, "max_rows must be positive, and experts * max_rows below 2^31");
   const c10::cuda::CUDAGuard guard(ids.device());
-  const auto i64 = ids.options().dtype(at::kLong);
-  at::Tensor pair_row = at::empty({ids.numel()}, i64), row_token = at::empty({experts * max_rows}, i64);
-  at::Tensor masked_m = at::empty({experts}, ids.options().dtype(at::kInt));
+  at::Tensor pair_row = empty({ids.numel()}, at::kLong, ids), row_token = empty({experts * max_rows}, at::kLong, ids);
+  at::Tensor masked_m = empty({experts}, at::kInt, ids);
   ag_route_layout_desc_t d{};
   d.max_rows = static_cast<int32_t>(max_rows);
   d.masked_m = static_cast<int32_t*>(masked_m.data_ptr());
@@ -267,10 +271,10 @@ std::tuple<at::Tensor, at::Tensor> combine_topk_backward(const at::Tensor& dy, c
   const c10::cuda::CUDAGuard guard(dy.device());
   at::Tensor drows, dweights, seen;
   if (need_rows) {
-    drows = at::empty_like(rows);
-    seen = at::empty({(rows.size(0) + 3) / 4 * 4}, rows.options().dtype(at::kByte));
+    drows = empty(rows.sizes(), rows.scalar_type(), rows);
+    seen = empty({(rows.size(0) + 3) / 4 * 4}, at::kByte, rows);
   }
-  if (need_weights) dweights = at::empty_like(weights);
+  if (need_weights) dweights = empty(weights.sizes(), at::kFloat, weights);
   check_ok(ag_combine_topk_backward(dy.data_ptr(), rows.data_ptr(), rows.scalar_type() == at::kFloat, rows.size(0),
                                     static_cast<const int64_t*>(ptr_of(pos)), static_cast<const float*>(weights.data_ptr()), dy.size(0),
                                     static_cast<int32_t>(weights.size(1)), dy.size(1), need_rows ? drows.data_ptr() : nullptr,
@@ -310,7 +314,7 @@ at::Tensor linear_workspace(ag_linear_desc_t& d, const at::Tensor& x, bool backw
   at::Tensor workspace;
   const uint64_t need = ag_linear_workspace_bytes(&d, backward);
   if (need > 0) {
-    workspace = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
+    workspace = empty({static_cast<int64_t>(need)}, at::kByte, x);
     d.workspace = workspace.data_ptr();
     d.workspace_bytes = need;
   }
@@ -337,11 +341,11 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
     d.ldr = row_stride(*residual);
   }
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor y = at::empty({d.m, d.n}, x.options().dtype(out_type)), pre;
+  at::Tensor y = empty({d.m, d.n}, out_type, x), pre;
   d.y = y.data_ptr();
   d.ldy = d.n;
   if (keep_pre) {
-    pre = at::empty({d.m, d.n}, x.options());
+    pre = empty({d.m, d.n}, x.scalar_type(), x);
     d.pre = pre.data_ptr();
     d.ldp = d.n;
   }
@@ -371,15 +375,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor&
   const c10::cuda::CUDAGuard guard(x.device());
   at::Tensor dx, dweight, dbias, workspace;
   if (need_x) {
-    dx = at::empty({d.m, d.k}, x.options());
+    dx = empty({d.m, d.k}, x.scalar_type(), x);
     d.dx = dx.data_ptr();
   }
   if (need_weight) {
-    dweight = at::empty({d.n, d.k}, x.options());
+    dweight = empty({d.n, d.k}, x.scalar_type(), x);
     d.dweight = dweight.data_ptr();
   }
   if (need_bias) {
-    dbias = at::empty({d.n}, x.options().dtype(bias_fp32 ? at::kFloat : x.scalar_type()));
+    dbias = empty({d.n}, bias_fp32 ? at::kFloat : x.scalar_type(), x);
     d.bias_dtype = bias_fp32 ? AG_T_FP32 : d.dtype;
     d.dbias = dbias.data_ptr();
   }
