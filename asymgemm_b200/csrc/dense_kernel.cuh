@@ -224,6 +224,12 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t smem_addr) {
 template <bool MN>
 __host__ __device__ constexpr int operand_k_bytes() { return MN ? 16 * 128 : 32; }
 
+// A wait of a whole warp with one answer for all of it: a lane that gave up takes the others along, so that they meet at the
+// warp's next synchronisation.
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, const WaitCtx& c, int code) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, c, code));
+}
+
 // One step of an operand: ROWS rows from `row`, contraction indices from `k`.
 template <bool MN, int ROWS>
 __device__ __forceinline__ void load_operand(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int k) {
@@ -357,7 +363,7 @@ dense_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const bool issuer = elect_one();
     for (int i = 0; i < steps; ++i) {
       const int s = i % ST;
-      if (!wait_bar(&empty[s], ((i / ST) & 1) ^ 1, wc, ST_TIMEOUT_A_EMPTY)) break;
+      if (!wait_bar_warp(&empty[s], ((i / ST) & 1) ^ 1, wc, ST_TIMEOUT_A_EMPTY)) break;
       if (!issuer) continue;
       mbar_arrive_expect_tx(&full[s], L::stage_bytes);
       uint8_t* dst = smem + s * L::stage_bytes;
@@ -369,8 +375,8 @@ dense_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     const uint64_t da0 = operand_desc<A_MN>(smem_u32(smem)), db0 = operand_desc<B_MN>(smem_u32(smem) + L::a_bytes);
     for (int i = 0, chunk = 0, j = 0; i < steps; ++i) {
       const int s = i % ST, slot = chunk & 1;
-      if (j == 0 && !wait_bar(&tm_empty[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY)) break;
-      if (!wait_bar(&full[s], (i / ST) & 1, wc, ST_TIMEOUT_A_FULL)) break;
+      if (j == 0 && !wait_bar_warp(&tm_empty[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY)) break;
+      if (!wait_bar_warp(&full[s], (i / ST) & 1, wc, ST_TIMEOUT_A_FULL)) break;
       tc_fence_after_sync();
       const uint64_t da = da0 + ((s * L::stage_bytes) >> 4), db = db0 + ((s * L::stage_bytes) >> 4);
       const bool last = j + 1 == p.chunk_steps || i == steps - 1;
@@ -405,8 +411,7 @@ dense_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     bool ok = true;
     for (int chunk = 0; chunk < chunks; ++chunk) {
       const int slot = chunk & 1;
-      ok = wait_bar(&tm_full[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_FULL);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = wait_bar_warp(&tm_full[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_FULL);
       if (!ok) break;
       tc_fence_after_sync();
       // once the last chunk is complete every load has landed and every MMA has read it, so the ring is free for the tile
@@ -593,7 +598,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const int a = item.a0 + static_cast<int>(rank) * 128, b = item.b0 + static_cast<int>(rank) * 128;
         for (int i = 0; i < item.steps; ++i, ++it) {
           const uint32_t s = it % ST;
-          ok = wait_bar(&empty[s], ((it / ST) & 1) ^ 1, wc, ST_TIMEOUT_A_EMPTY);
+          ok = wait_bar_warp(&empty[s], ((it / ST) & 1) ^ 1, wc, ST_TIMEOUT_A_EMPTY);
           if (!ok) break;
           const uint32_t bar = map_to_cta(smem_u32(&full[s]), 0);
           uint8_t* dst = smem + s * L::stage_bytes;
@@ -626,9 +631,9 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const PairItem item = pair_item(params, w, tiles_a, splits);
         for (int i = 0, j = 0; i < item.steps; ++i, ++it) {
           const uint32_t s = it % ST, slot = chunk & 1;
-          if (j == 0) ok = wait_bar(&tm_empty[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY) &&
-                           wait_bar(&tm_empty_peer[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY);
-          if (ok) ok = wait_bar(&full[s], (it / ST) & 1, wc, ST_TIMEOUT_A_FULL);
+          if (j == 0) ok = wait_bar_warp(&tm_empty[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY) &&
+                           wait_bar_warp(&tm_empty_peer[slot], ((chunk >> 1) & 1) ^ 1, wc, ST_TIMEOUT_TM_EMPTY);
+          if (ok) ok = wait_bar_warp(&full[s], (it / ST) & 1, wc, ST_TIMEOUT_A_FULL);
           if (!ok) break;
           tc_fence_after_sync();
           const uint64_t da = da0 + ((s * L::stage_bytes) >> 4), db = db0 + ((s * L::stage_bytes) >> 4);
@@ -659,7 +664,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         const int chunks = ONE_CHUNK ? 1 : (item.steps + params.chunk_steps - 1) / params.chunk_steps;
         for (int c = 0; c < chunks && ok; ++c, ++chunk) {
           const uint32_t slot = chunk & 1;
-          ok = wait_bar(&tm_empty[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_EMPTY);
+          ok = wait_bar_warp(&tm_empty[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_EMPTY);
           if (ok && lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tm_empty_peer[slot]), 0));
           __syncwarp();
         }
@@ -686,8 +691,7 @@ dense_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
       uint32_t slot = 0;
       for (int c = 0; c < chunks; ++c, ++chunk) {
         slot = chunk & 1;
-        ok = wait_bar(&tm_full[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_FULL);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = wait_bar_warp(&tm_full[slot], (chunk >> 1) & 1, wc, ST_TIMEOUT_TM_FULL);
         if (!ok) break;
         tc_fence_after_sync();
         if constexpr (!ONE_CHUNK) {

@@ -80,6 +80,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act
             raise RuntimeError("x is [..., k] and dy [..., n] with the same leading dimensions")
         x, dy = x.reshape(-1, shape[-1]), dy.reshape(-1, dy.shape[-1])
         pre = pre.reshape(-1, pre.shape[-1]) if pre is not None else None
+    if dy.dim() == 2 and dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]:      # an expanded gradient, e.g. of a sum
+        dy = dy.contiguous()
     dx, dweight, dbias = _lib.torch_ops().linear_backward(dy, x, weight, act, pre, bool(need_x), bool(need_weight), bool(need_bias),
                                                           bias_dtype == torch.float32, api._status_word(x.device), api._state["timeout_ms"])
     return dx.view(shape) if dx is not None else None, dweight, dbias
@@ -104,7 +106,5 @@ class _Linear(torch.autograd.Function):
         dx = dweight = dbias = None
         if any(need[:3]):
             rows = dy if dy.stride(-1) == 1 or dy.shape[-1] == 1 else dy.contiguous()
-            if rows.dim() == 2 and rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:      # an expanded gradient, e.g. of a sum
-                rows = rows.contiguous()
             dx, dweight, dbias = linear_backward(rows, x, weight, ctx.act, pre, need[0], need[1], need[2], ctx.bias_dtype)
         return dx, dweight, dbias, dy if need[3] else None, None, None

@@ -213,6 +213,9 @@ def test_autograd_gives_the_same_gradients(activation):
     y.sum().backward()
     plain = torch.autograd.grad(dense_ops.linear(leaves[0].reshape(36, 72), leaves[1], activation=activation), leaves[1], torch.ones(36, 50, device=DEV, dtype=torch.bfloat16))
     assert torch.equal(leaves[1].grad, plain[0])
+    y = dense_ops.linear(leaves[0], leaves[1], activation=activation)
+    wide = torch.autograd.grad(y, leaves[1], torch.ones((1, 1, 50), device=DEV, dtype=torch.bfloat16).expand(4, 9, 50))
+    assert torch.equal(wide[0], plain[0])
     y = dense_ops.linear(leaves[0].reshape(36, 72), leaves[1], activation=activation)
     turned = torch.autograd.grad(y, leaves[1], randn(50, 36, seed=35).t(), retain_graph=True)[0]
     straight = torch.autograd.grad(y, leaves[1], randn(50, 36, seed=35).t().contiguous())[0]
@@ -254,6 +257,20 @@ def test_refusals():
     pinned = torch.empty((32, 64), dtype=torch.bfloat16).pin_memory()
     with pytest.raises(RuntimeError):
         dense_ops.linear(x, pinned)
+
+
+def test_the_result_may_take_the_residuals_place_through_the_c_abi():
+    from asymgemm_b200 import _lib
+    lib = _lib.load()
+    for m, n, k in ((30, 200, 512), (1000, 1536, 256), (40, 90, 136)):
+        x, w, r = randn(m, k, seed=36), randn(n, k, seed=37, scale=k ** -0.5), randn(m, n, seed=38)
+        want = dense_ops.linear(x, w, residual=r, activation="silu")
+        d = _lib.LinearDesc(m=m, n=n, k=k, activation=3, x=x.data_ptr(), weight=w.data_ptr(), residual=r.data_ptr(), y=r.data_ptr(), ldx=k, ldw=k, ldr=n, ldy=n,
+                            stream=torch.cuda.current_stream().cuda_stream)
+        space = torch.empty(max(1, int(lib.ag_linear_workspace_bytes(d, 0))), dtype=torch.uint8, device=DEV)
+        d.workspace, d.workspace_bytes = space.data_ptr(), space.numel()
+        _lib.check(lib.ag_linear(d))
+        assert torch.equal(r, want)
 
 
 def test_two_streams_and_two_captured_graphs_at_once():

@@ -425,12 +425,13 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------------------ together
-def test_route_layout_and_combine_together_in_a_captured_graph():
+@pytest.mark.parametrize("tokens,k", [(300, 4), (3000, 9)])
+def test_route_layout_and_combine_together_in_a_captured_graph(tokens, k):
     """Logits -> ids, weights -> layout -> rows gathered, scaled by expert (in place of the experts' products) -> combine, and
     the way back to the logits, replayed on new inputs."""
-    tokens, experts, k, cols = 300, 24, 4, 256
+    experts, cols, live = 24, 256, tokens - 20
     x, logits = randn(tokens, cols, seed=60, dtype=torch.bfloat16, scale=1.0), randn(tokens, experts, seed=61)
-    used = torch.tensor([280], dtype=torch.int32, device=DEV)
+    used = torch.tensor([live], dtype=torch.int32, device=DEV)
     dy = randn(tokens, cols, seed=62, dtype=torch.bfloat16, scale=1.0)
 
     def step():
@@ -454,8 +455,8 @@ def test_route_layout_and_combine_together_in_a_captured_graph():
         for got, w in zip(out, want):
             assert torch.equal(got, w)
     # every token's rows are its own x: the combine gives x back where the weights sum to 1
-    y, xs = out[2][:280].double(), x[:280].double()
-    assert bool(((y - xs).abs() <= xs.abs() * (2 ** -8 + 16 * 2 ** -22)).all()) and float(out[2][280:].abs().max()) == 0
+    y, xs = out[2][:live].double(), x[:live].double()
+    assert bool(((y - xs).abs() <= xs.abs() * (2 ** -8 + 16 * 2 ** -22)).all()) and float(out[2][live:].abs().max()) == 0
 
 
 @pytest.mark.parametrize("tokens,experts,k,cols,dtype", [(37, 8, 3, 64, torch.bfloat16), (1, 256, 8, 32, torch.bfloat16), (700, 60, 4, 20, torch.float32)])
