@@ -740,7 +740,8 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
 //   renormalised:  dl_i = scale * q_i * d_i * (g_i - sum_j q_j g_j),  q = s / S,  d = 1 (softmax) or 1 - s_i (sigmoid);
 //   sigmoid:       dl_i = scale * g_i * s_i * (1 - s_i);
 //   softmax:       dl_j = scale * s_j * ([j chosen] g_j - sum_i s_i g_i), for every expert j.
-// Experts that do not appear get 0, so only the last form reads the whole row; all write it, once, in 16-byte pieces.
+// Experts that do not appear get 0, so only the last form reads the whole row; all write it in 16-byte pieces and the few chosen
+// entries over it (65536 x 256 fp32, top 8: 42 us with the entries merged into the pieces before the store, 24 so).
 struct RouteGradParams {
   const void* logits;
   const float* dweights;
@@ -803,35 +804,37 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
     dot = warp_sum_f(s * g);
     v = s * g;
   }
+  // an expert named twice in a row gets both parts, from the first lane that names it
+  const unsigned same = __match_any_sync(kAll, id);
+  if (__any_sync(kAll, id >= 0 && __popc(same) > 1)) {
+    float all = 0.f;
+    for (int t = 0; t < p.top_k; ++t) {
+      const float other = __shfl_sync(kAll, v, t);
+      if (same >> t & 1u) all += other;
+    }
+    if (id >= 0) v = all;
+  }
+  // the row as it is without the chosen experts, then the chosen ones over it
   constexpr int V = VECTOR ? 16 / static_cast<int>(sizeof(T)) : 1;      // elements a lane writes at once
-  for (int first = 0; first < p.experts; first += 32 * V) {            // every lane of the warp takes every round
-    const int e0 = first + lane * V;
-    float a[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      a[i] = 0.f;
-      if (dense && e0 + i < p.experts) {
-        const float x = clean(to_float(row[e0 + i]));
-        if (x > -INFINITY) a[i] = -expf(x - row_max) * inv * dot;
-      }
-    }
-    for (int t = 0; t < p.top_k; ++t) {      // an expert named twice in a row gets both parts
-      const int at = __shfl_sync(kAll, id, t) - e0;
-      const float add = __shfl_sync(kAll, v, t);
-#pragma unroll
-      for (int i = 0; i < V; ++i) a[i] += at == i ? add : 0.f;
-    }
-    if (e0 >= p.experts) continue;
+  auto rest = [&](int e) {
+    const float x = clean(to_float(row[e]));
+    return x > -INFINITY ? -expf(x - row_max) * inv * dot : 0.f;
+  };
+  for (int e0 = lane * V; e0 < p.experts; e0 += 32 * V) {
     if constexpr (VECTOR) {
-      uint4 o;
-      T* t = reinterpret_cast<T*>(&o);
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (dense) {
+        T* t = reinterpret_cast<T*>(&o);
 #pragma unroll
-      for (int i = 0; i < V; ++i) t[i] = from_float<T>(a[i]);
+        for (int i = 0; i < V; ++i) t[i] = from_float<T>(rest(e0 + i));
+      }
       *reinterpret_cast<uint4*>(out + e0) = o;
     } else {
-      out[e0] = from_float<T>(a[0]);
+      out[e0] = from_float<T>(dense ? rest(e0) : 0.f);
     }
   }
+  __syncwarp();
+  if (id >= 0 && lane == __ffs(same) - 1) out[id] = from_float<T>(dense ? v + rest(id) : v);
 }
 
 // ------------------------------------------------------------------------------------------------ layout tables
@@ -868,7 +871,6 @@ __device__ __forceinline__ int pair_expert(const LayoutParams& p, long long i, b
 
 __global__ void __launch_bounds__(kLayoutThreads) layout_count_kernel(const LayoutParams p) {
   extern __shared__ int count[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the next kernel starts on its own pairs meanwhile
   for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) count[e] = 0;
   __syncthreads();
   const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
@@ -920,15 +922,14 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
     }
   }
   if (!ONE) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");      // the counts are complete
     // all blocks' counts, `parts` threads per expert; integer sums, so their order does not matter
     const int parts = max(1, kLayoutThreads / E);
     for (int i = threadIdx.x; i < parts * E; i += kLayoutThreads) {
       const int e = i % E;
       int all = 0, before = 0;
-#pragma unroll 16
+#pragma unroll 8
       for (int b = i / E; b < static_cast<int>(gridDim.x); b += parts) {
-        const int v = __ldcg(p.block_counts + static_cast<long long>(b) * E + e);
+        const int v = __ldg(p.block_counts + static_cast<long long>(b) * E + e);
         all += v;
         before += b < static_cast<int>(blockIdx.x) ? v : 0;
       }
@@ -1235,20 +1236,7 @@ int ag_route_layout(const ag_route_layout_desc_t* r) {
     if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   }
   if (blocks > 1) agb::layout_count_kernel<<<blocks, agb::kLayoutThreads, static_cast<size_t>(r->experts) * 4, stream>>>(p);
-  // Launched while the counting kernel runs: it counts its own pairs before it waits for the others' counts. It writes nothing
-  // but shared memory and the status word before that.
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(agb::kLayoutThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = blocks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, place, p);
-  if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
+  place<<<blocks, agb::kLayoutThreads, smem, stream>>>(p);
   return launch_check();
 }
 
