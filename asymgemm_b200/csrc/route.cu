@@ -95,11 +95,11 @@ struct Slots {
   }
 };
 
-// The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left). Every loop is rolled: the code runs for
-// a handful of rows per SM, so what it costs is fetching its instructions (unrolled, the 65536 x 256 case took 58 us instead of
-// 47).
+// The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left). Every loop is rolled: it runs for a few
+// rows per million, and its size is all that the others see of it (65536 x 256: 53 us inlined so, 57 as a called function, whose
+// calling convention the whole kernel pays for).
 template <typename T>
-__device__ __noinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
+__device__ __forceinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
   const Slots at(p, p.warp, lane);
   double c[kRouteMaxPerLane], mx = -INFINITY, sum = 0;
   auto logit = [&](int j) { return static_cast<double>(clean(to_float(row[at.first + j]))); };
@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(128) route_topk_kernel(const RouteParams p) {
 // larger of a[i] and b[7 - i] are the 8 best of both, in bitonic order), after which every lane of the row has the answer
 // without a serial step per expert. The best key that a merge leaves out is kept: it says whether the eighth is clear of the rest.
 // Experts too close for their keys (the index takes 8 of 24 bits with 256 experts, so one token in twenty) are put in order by
-// their exact values, one per lane; only where the border itself is unclear does route_exact decide the row.
+// their fp32 values, one per lane, and where those are too close by 64-bit ones; only where several more than eight are close at
+// the border, or two groups are, does route_exact decide the row.
 __device__ __forceinline__ void bitonic8(int32_t (&a)[8]) {
 #pragma unroll
   for (int d = 4; d > 0; d >>= 1) {
@@ -466,7 +467,7 @@ __device__ __forceinline__ void load8(bool vector, const T* mine, int count, int
 
 // Rolled over a lane's pieces of 8 experts: straight-line code for 32 of them did not fit the instruction cache. STAGED: the warp's rows come through shared memory by 16-byte asynchronous copies, each lane's
 // experts 16 bytes further apart there; read straight from memory, lanes 64 bytes or more apart take a cache line each for 16
-// bytes (65536 x 256 fp32: 57 us so, with that and the 64-bit comparison of every close pair).
+// bytes.
 template <typename T, bool STAGED>
 __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31, width = p.row_lanes, in_row = lane & (width - 1), row0 = lane & ~(width - 1);
@@ -537,12 +538,8 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
   const int32_t index_mask = (1 << p.index_bits) - 1;
   int32_t top[8], left = INT32_MIN;
   float a1 = -INFINITY, a2 = -INFINITY;
-  float c[8];
-  load8<T, true>(p.part.vector_rows, mine, at.count, 0, c);
-#pragma unroll 1
-  for (int q = 0; q < pieces; ++q) {
-    float s[8], next[8];
-    if (q + 1 < pieces) load8<T, true>(p.part.vector_rows, mine, at.count, q + 1, next);
+  // One piece: c raw logits in, cleaned ones out, s the scores with their bias (where scores are needed).
+  auto score = [&](int q, float (&c)[8], float (&s)[8]) {
     // NaN, infinities and missing experts are rare: one look at the sum spares the common piece two operations per expert
     float size = 0.f;
 #pragma unroll
@@ -558,25 +555,34 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[j] = clean(c[j]);
     }
+    if (!scored) return;
+    if (p.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = reciprocal(1.f + __expf(-c[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = __expf(c[j] - row_max) * inv;
+    }
+    if (special) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
+        if (p.bias != nullptr) b[j] = clean(b[j]);
+      }
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += b[j];      // a bias of -inf switches the expert off by itself
+    }
+  };
+  float c[8];
+  load8<T, true>(p.part.vector_rows, mine, at.count, 0, c);
+#pragma unroll 1
+  for (int q = 0; q < pieces; ++q) {
+    float s[8], next[8];
+    if (q + 1 < pieces) load8<T, true>(p.part.vector_rows, mine, at.count, q + 1, next);
+    score(q, c, s);
     if (scored) {
-      if (p.sigmoid) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = reciprocal(1.f + __expf(-c[j]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = __expf(c[j] - row_max) * inv;
-      }
-      if (special) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          s[j] = c[j] == -INFINITY ? -INFINITY : s[j];
-          if (p.bias != nullptr) b[j] = clean(b[j]);
-        }
-      }
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] += b[j];      // a bias of -inf switches the expert off by itself
-      }
       if (p.groups > 1) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -610,7 +616,7 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
     for (int j = 0; j < 8; ++j) c[j] = next[j];
   }
 
-  bool unsure = false;
+  bool unsure = false, kept = true;
   if (p.groups > 1) {
     for (int o = 1; o < (1 << p.part.shift); o <<= 1) {
       const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
@@ -624,7 +630,8 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
       const float other = __shfl_sync(kAll, mine, row0 + (o << p.part.shift));
       rank += other > mine || (other == mine && o < g);
     }
-    const bool kept = rank < p.top_groups, real = g < p.groups;
+    const bool real = g < p.groups;
+    kept = rank < p.top_groups;
     // the weakest group kept against the strongest one left out
     const float low = -row_max_of(real && kept ? -mine : -INFINITY), high = row_max_of(real && !kept ? mine : -INFINITY);
     if (high > -INFINITY) unsure = !(low - high > 4.f * tol + 0x1p-20f * (fabsf(low) + fabsf(high)));
@@ -658,22 +665,46 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
     const unsigned all_close = __ballot_sync(kAll, close);
     if (all_close != 0u) {
       const unsigned here = (all_close >> row0) & 0xffu;
-      // what was left out may belong among the first top_k only if nothing separates it from them
+      // what was left out may belong among the first top_k only if nothing separates it from them; then the best one left out
+      // takes part below, and if the row has more that close, route_exact decides it
       const unsigned chain = 0xffu & ~((1u << (p.top_k - 1)) - 1u);
-      unsure = unsure || (here & chain) == chain;
+      bool border = (here & chain) == chain;
+      if (__any_sync(kAll, border)) {
+        const float last = value_of(__shfl_sync(kAll, key, row0 + 7) & ~index_mask), least = last - 2.f * off - cut * 2.f * fabsf(last);
+        int near = 0;
+#pragma unroll 1
+        for (int q = 0; q < pieces; ++q) {
+          float s[8];
+          load8<T, true>(p.part.vector_rows, mine, at.count, q, c);
+          score(q, c, s);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) near += kept && (p.bias != nullptr ? s[j] : c[j]) >= least;
+        }
+        for (int o = width >> 1; o > 0; o >>= 1) near += __shfl_xor_sync(kAll, near, o);
+        if (border && near > 9) {
+          unsure = true;
+          border = false;
+        }
+      }
+      const int ninth = border ? expert_of(left) : -1;
       // in order by the whole fp32 value, then, where even that is within its error of the next, by the exact one
       const float l = chosen >= 0 ? logit(chosen) : -INFINITY, b = p.bias != nullptr && chosen >= 0 ? clean(p.bias[chosen]) : 0.f;
-      float f = l;
-      if (p.bias != nullptr && chosen >= 0) f = (p.sigmoid ? __fdividef(1.f, 1.f + __expf(-l)) : __expf(l - row_max) * inv) + b;
-      auto sort_by = [&](auto value) {
-        int rank = 0;
+      const float l9 = ninth >= 0 ? logit(ninth) : -INFINITY, b9 = p.bias != nullptr && ninth >= 0 ? clean(p.bias[ninth]) : 0.f;
+      auto value32 = [&](float l, float b) {
+        return p.bias == nullptr || l == -INFINITY ? l : (p.sigmoid ? reciprocal(1.f + __expf(-l)) : __expf(l - row_max) * inv) + b;
+      };
+      const float f = value32(l, b), f9 = value32(l9, b9);
+      // the eight, and the ninth where there is one, by value and then by index; lane i gets the i-th
+      auto sort_by = [&](auto value, auto value9) {
+        int rank = ninth >= 0 && (value9 > value || (value9 == value && ninth < chosen)), rank9 = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const auto v = __shfl_sync(kAll, value, row0 + j);
           const int e = __shfl_sync(kAll, chosen, row0 + j);
           rank += v > value || (v == value && e < chosen);
+          rank9 += v > value9 || (v == value9 && e < ninth);
         }
-        int sorted = -1;
+        int sorted = ninth >= 0 && rank9 == in_row ? ninth : -1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int r = __shfl_sync(kAll, rank, row0 + j), e = __shfl_sync(kAll, chosen, row0 + j);
@@ -683,18 +714,19 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
       };
       // two with the same logit and bias are in the right order already, by index, and need no more
       bool alike = false;
+      auto compare = [&](float fj, float lj, float bj) {
+        alike = alike || (in_row < 8 && chosen >= 0 && lj > -INFINITY && (lj != l || bj != b) && !(fabsf(fj - f) > 2.f * off + 0x1p-22f * (fabsf(fj) + fabsf(f))));
+      };
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float fj = __shfl_sync(kAll, f, row0 + j), lj = __shfl_sync(kAll, l, row0 + j), bj = __shfl_sync(kAll, b, row0 + j);
-        alike = alike || (in_row < 8 && chosen >= 0 && (lj != l || bj != b) && lj > -INFINITY && !(fabsf(fj - f) > 2.f * off + 0x1p-22f * (fabsf(fj) + fabsf(f))));
-      }
+      for (int j = 0; j < 8; ++j) compare(__shfl_sync(kAll, f, row0 + j), __shfl_sync(kAll, l, row0 + j), __shfl_sync(kAll, b, row0 + j));
+      compare(f9, l9, b9);
       alike = alike && p.bias != nullptr;      // logits alone are exact
-      int sorted = sort_by(f);
+      int sorted = sort_by(f, f9);
       const unsigned all_alike = __ballot_sync(kAll, alike);
       if (all_alike != 0u) {
         if (p.sigmoid) {
-          const double d = chosen >= 0 ? 1 / (1 + exp(-static_cast<double>(l))) + static_cast<double>(b) : -INFINITY;
-          sorted = sort_by(d);
+          auto value64 = [&](float l, float b) { return l > -INFINITY ? 1 / (1 + exp(-static_cast<double>(l))) + static_cast<double>(b) : -INFINITY; };
+          sorted = sort_by(value64(l, b), value64(l9, b9));
         } else if (((all_alike >> row0) & 0xffu) != 0u) {
           unsure = true;      // a softmax score needs its sum in 64 bits too
         }

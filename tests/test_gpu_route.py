@@ -140,6 +140,31 @@ def test_scores_that_fp32_cannot_tell_apart_are_ordered_as_in_64_bits():
     check_route(torch.linspace(-60, 0, experts).repeat(4, 1).to(DEV), 8, scoring="softmax", bias=torch.zeros(experts, device=DEV))
 
 
+@pytest.mark.parametrize("k", [1, 5, 8, 12])
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 4)])
+def test_two_experts_that_meet_at_the_border(k, groups, top_groups):
+    """In every row the expert that is just chosen and the one that is just left out differ by 0 to a few hundred steps of fp32."""
+    gen = torch.Generator().manual_seed(k + groups)
+    tokens, experts = 640, 128
+    logits = torch.randn((tokens, experts), generator=gen) * 1.5
+    bias = torch.randn(experts, generator=gen) * 0.05
+    step = torch.randint(-400, 401, (tokens,), generator=gen).double() * 2.0 ** -26 * torch.randint(0, 2, (tokens,), generator=gen)
+    # among equals in the same groups: the reference's own order says which experts stand at the border
+    order = plain_route(logits, k + 1, "sigmoid", bias, groups, top_groups)[0]
+    at, out = order[:, k - 1], order[:, k]
+    rows = torch.arange(tokens)
+    choice = torch.sigmoid(logits[rows, at].double()) + bias[at].double() + step
+    wanted = (choice - bias[out].double()).clamp(1e-3, 1 - 1e-3)
+    logits[rows, out] = torch.log(wanted / (1 - wanted)).float()
+    check_route(logits.to(DEV), k, scoring="sigmoid", bias=bias.to(DEV), num_groups=groups, top_groups=top_groups)
+    # logits alone: neighbours in fp32, and equal ones
+    order = plain_route(logits, k + 1, "softmax", None, groups, top_groups, "max")[0]
+    at, out = order[:, k - 1], order[:, k]
+    logits[rows, out] = torch.nextafter(logits[rows, at], torch.where(rows % 3 == 0, logits[rows, at], torch.where(rows % 3 == 1, 1e9, -1e9)))
+    check_route(logits.to(DEV), k, num_groups=groups, top_groups=top_groups, group_score="max")
+    check_route(logits.to(DEV), k, scoring="softmax", bias=torch.zeros(experts, device=DEV), num_groups=groups, top_groups=top_groups, group_score="max")
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_experts_that_are_off_and_values_without_end(scoring):
     logits = randn(12, 48, seed=11)
