@@ -1219,7 +1219,7 @@ uint64_t ag_route_layout_workspace_bytes(int64_t pairs, int32_t experts) {
 
 int ag_route_layout(const ag_route_layout_desc_t* r) {
   if (r == nullptr) return agb_fail(AG_E_INVALID, "desc is NULL");
-  if (r->tokens < 0 || r->top_k <= 0 || r->experts <= 0 || r->experts > agb::kLayoutMaxExperts || r->max_rows < 0 || r->rows < 0)
+  if (r->tokens < 0 || r->tokens > 0x7fffffffLL || r->top_k <= 0 || r->experts <= 0 || r->experts > agb::kLayoutMaxExperts || r->max_rows < 0 || r->rows < 0)
     return agb_fail(AG_E_INVALID, "bad sizes (at most 1024 experts)");
   const int64_t pairs = r->tokens * r->top_k;
   if (pairs > 0x7fffffffLL / 2 || r->rows > 0x7fffffffLL) return agb_fail(AG_E_INVALID, "too many (token, slot) pairs");

@@ -3,7 +3,8 @@ besides its experts -- router logits, shared experts, projections -- with the we
 memory are the grouped GEMMs' business: a single dense product would read them at the host link's rate.)
 
 The kernels are tcgen05 products fed by TMA, so rows of `x` and `weight` start on 16-byte boundaries: k is a multiple of 8.
-Everything runs on the current stream; there is no CPU branch.
+Everything runs on the current stream; there is no CPU branch. `linear` is recorded by autograd; `linear_backward` is the same
+gradient as a function of its own, which is the form to capture into a CUDA graph.
 """
 from __future__ import annotations
 

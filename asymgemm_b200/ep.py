@@ -275,7 +275,7 @@ class EPDispatcher:
             main.wait_stream(comm)
         inv = torch.empty_like(order)
         inv[order] = torch.arange(order.numel(), device=dev)
-        y = moe_ops.combine_topk(ret_sorted, inv, topk_weights, tokens, top_k)
+        y = moe_ops.combine_topk_forward(ret_sorted, inv, topk_weights, tokens, top_k)
         del keep
         return y
 
@@ -292,7 +292,7 @@ class EPDispatcher:
         if state.tables is not None:
             if mark is not None:
                 mark("return")
-            return moe_ops.combine_topk(expert_out, state.tables.pair_row, topk_weights, state.tokens, state.top_k)
+            return moe_ops.combine_topk_forward(expert_out, state.tables.pair_row, topk_weights, state.tokens, state.top_k)
         # inverse of the sort: pair p (token p // k, slot p % k) was sent as sorted row inv[p]
         inv = torch.empty_like(state.order)
         inv[state.order] = torch.arange(state.order.numel(), device=state.order.device)
@@ -301,13 +301,13 @@ class EPDispatcher:
             pos = state.dest_rows.index_select(0, inv)
             if mark is not None:
                 mark("return")
-            return moe_ops.combine_topk(expert_out, pos, topk_weights, state.tokens, state.top_k)
+            return moe_ops.combine_topk_forward(expert_out, pos, topk_weights, state.tokens, state.top_k)
         back = moe_ops.move_rows(expert_out, state.dest_rows.numel(), src_rows=state.dest_rows)
         ret = torch.empty((state.tokens * state.top_k, back.shape[1]), dtype=back.dtype, device=back.device)
         self._all_to_all(ret, back, state.send_splits, state.recv_splits)
         if mark is not None:
             mark("return")
-        return moe_ops.combine_topk(ret, inv, topk_weights, state.tokens, state.top_k)
+        return moe_ops.combine_topk_forward(ret, inv, topk_weights, state.tokens, state.top_k)
 
 
 def to_contiguous_layout(recv: torch.Tensor, state: DispatchState) -> torch.Tensor:
@@ -576,7 +576,7 @@ class ExpertParallelMoE:
             api.prefetch_weights(self.prefetch_next, out.device)
         if px.pair_row is not None:      # one rank: every result already lies in this rank's memory
             self._mark("return")
-            y = moe_ops.combine_topk(out, px.pair_row, topk_weights, tokens, top_k)
+            y = moe_ops.combine_topk_forward(out, px.pair_row, topk_weights, tokens, top_k)
             self._mark("combine")
             return y
         if direct:
@@ -584,7 +584,7 @@ class ExpertParallelMoE:
         else:
             px.send_back(out)
         self._mark("return")
-        y = moe_ops.combine_topk(px.ret.view(torch.bfloat16).view(px.pairs_cap, self.hidden), None, topk_weights, tokens, top_k)
+        y = moe_ops.combine_topk_forward(px.ret.view(torch.bfloat16).view(px.pairs_cap, self.hidden), None, topk_weights, tokens, top_k)
         self._mark("combine")
         return y
 

@@ -130,14 +130,18 @@ def move_rows_into(out: torch.Tensor, src: torch.Tensor, dst_rows: torch.Tensor)
 
 def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (CUDA: bf16); pos None =
-    t*top_k + j. On CUDA slots with a negative pos (pairs a layout dropped) add nothing, and the call is differentiable with
-    respect to `rows` and `weights`; a row that two slots name has no gradient (see `combine_topk_backward`)."""
-    if rows.is_cuda and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
+    `weights`; where the CUDA kernels run (contiguous rows, bf16 with cols a multiple of 8 or fp32 with a multiple of 4) the
+    gradient is `combine_topk_backward`'s: no two slots may name the same row, and cols must be a multiple of 8."""
+    kernel = rows.is_cuda and rows.is_contiguous() and rows.shape[1] % {torch.bfloat16: 8, torch.float32: 4}.get(rows.dtype, 1 << 62) == 0
+    if kernel and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
-    return _combine_topk(rows, pos, weights, tokens, top_k)
+    return combine_topk_forward(rows, pos, weights, tokens, top_k)
 
 
-def _combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
+def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
+    """`combine_topk` without a record for autograd where the CUDA kernels run: the layers' inference path, whose GEMMs have none
+    either and whose buffers the next call overwrites."""
     cols = rows.shape[1]
     if tokens == 0:
         return torch.empty((0, cols), dtype=torch.bfloat16 if rows.is_cuda else rows.dtype, device=rows.device)
@@ -179,12 +183,14 @@ class _CombineTopK(torch.autograd.Function):
     def forward(ctx, rows, pos, weights, tokens, top_k):
         ctx.save_for_backward(rows, pos, weights)
         ctx.top_k = top_k
-        return _combine_topk(rows, pos, weights, tokens, top_k)
+        return combine_topk_forward(rows, pos, weights, tokens, top_k)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         rows, pos, weights = ctx.saved_tensors
+        if pos is not None:
+            pos = pos[: weights.numel()]      # a table may be longer than the batch
         drows, dweights = combine_topk_backward(dy.contiguous(), rows, pos, weights.reshape(dy.shape[0], ctx.top_k), ctx.needs_input_grad[0],
                                                 ctx.needs_input_grad[2])
         if dweights is not None:

@@ -386,6 +386,46 @@ def test_gradient_of_the_combine(tokens, experts, k, cols, dtype):
     assert torch.equal(got[0], drows) and torch.equal(got[1], dweights)
 
 
+def test_gradient_of_the_combine_where_plain_torch_computes_it():
+    """Types and widths without a kernel: float16, and bf16 rows of 12 columns."""
+    for dtype, cols in ((torch.float16, 64), (torch.bfloat16, 12)):
+        lay, rows, weights, _ = combine_case(9, 4, 2, cols, dtype, 33)
+        a, b = rows.clone().requires_grad_(True), weights.clone().requires_grad_(True)
+        y = moe_ops.combine_topk(a, lay.pair_row, b, 9, 2)
+        dy = randn(9, cols, seed=34, dtype=dtype, scale=1.0)
+        drows, dweights = torch.autograd.grad(y, (a, b), dy)
+        pos = lay.pair_row.cpu()
+        live = pos >= 0
+        g, w = dy.cpu().double().repeat_interleave(2, 0), weights.cpu().double().view(-1, 1)
+        want = torch.zeros(rows.shape, dtype=torch.float64)
+        want[pos[live]] = (w * g)[live]
+        assert bool(((drows.cpu().double() - want).abs() <= want.abs() * (torch.finfo(dtype).eps / 2 + 2 ** -23)).all())
+        terms = torch.where(live.view(-1, 1), rows.cpu().double()[pos.clamp(min=0)] * g, 0)
+        # a product and at most `cols` additions in fp32
+        assert bool(((dweights.cpu().double().view(-1) - terms.sum(1)).abs() <= terms.abs().sum(1) * (cols + 1) * 2 ** -24).all())
+
+
+def test_position_tables_may_be_longer_than_the_batch():
+    lay, rows, weights, dy = combine_case(11, 4, 2, 64, torch.bfloat16, 35)
+    longer = torch.cat([lay.pair_row, torch.full((9,), 5, device=DEV)])
+    grads = []
+    for pos in (lay.pair_row, longer):
+        a, b = rows.clone().requires_grad_(True), weights.clone().requires_grad_(True)
+        grads.append(torch.autograd.grad(moe_ops.combine_topk(a, pos, b, 11, 2), (a, b), dy))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+def test_layers_record_no_gradient():
+    """The layers' GEMMs have no gradient, so their output claims none either, whatever the weights ask for."""
+    from asymgemm_b200.ep import EPDispatcher
+    disp = EPDispatcher(8)
+    ids, x, w = make_ids(20, 8, 2, 36).to(DEV), randn(20, 64, seed=37, dtype=torch.bfloat16), torch.rand((20, 2), device=DEV, requires_grad=True)
+    state, _, _ = disp.dispatch(x, ids)
+    out = randn(state.padded_rows, 64, seed=38, dtype=torch.bfloat16)
+    assert not disp.combine(out, state, w).requires_grad
+    assert moe_ops.combine_topk(out, state.tables.pair_row, w, 20, 2).requires_grad
+
+
 def test_gradient_of_the_combine_without_a_position_table():
     rows, w = randn(60, 256, seed=40, dtype=torch.bfloat16), torch.rand((20, 3), device=DEV)
     dy = randn(20, 256, seed=41, dtype=torch.bfloat16)
