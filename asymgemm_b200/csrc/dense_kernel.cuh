@@ -253,7 +253,8 @@ __device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[VW]) {
 // ------------------------------------------------------------------------------------------------ one tile per CTA
 // 128 x BN tile per CTA, the contraction split over the CTAs of a cluster (1, 2, 4 or 8). The CTAs' partial tiles meet in
 // shared memory: each sums an equal share of the tile over the cluster in the order of the splits (so the result does not
-// depend on timing), applies the epilogue and stores it. No workspace, no atomics, one launch.
+// depend on timing), applies the epilogue and stores it. No workspace, no atomics, one launch. Measured: 64 x 7168 x 2048
+// 10.0 us, 4 x 256 x 7168 8.6, 128 x 1024 x 512 6.7: launch, pipeline fill, join and epilogue are most of these.
 template <int BN>
 constexpr int tile_stages() { return BN >= 128 ? 6 : BN == 64 ? 4 : 5; }   // BN <= 64: two CTAs fit on an SM
 
@@ -464,6 +465,9 @@ dense_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 // operands in L2. The drain's last pass over a tile -- bias, activation, residual, stores -- runs while the MMAs fill the
 // two TMEM buffers of the next tile.
 // With splits > 1 every split writes its fp32 partial to a workspace plane of its own and join_splits_kernel adds them in order.
+// Measured: 8192 x 4096 x 7168 bf16 with silu 312 us (1540 TFLOP/s) in short runs, 388 under the power cap; 16384 x 256 x 7168 with
+// fp32 outputs 57 us (39 of memory traffic; 64 tiles on 74 pairs, which pull 695 MB through L2); 2048 x 256 x 65536 split over 8:
+// 62 us and 8 more for the join.
 constexpr int kPairTile = 256, kPairStages = 6, kPairRowBlock = 8;
 struct PairDenseSmem {
   static constexpr int box_bytes = 128 * 128;                    // one CTA's 128 rows of an operand, one step

@@ -12,7 +12,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from . import _lib
+from . import _lib, api
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
@@ -46,7 +46,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 
 def _forward(x, weight, bias, residual, act, out_dtype, keep_pre):
-    from . import api
     flat = x.dim() == 2
     if not flat:
         shape = x.shape[:-1] + (weight.shape[0],)
@@ -70,7 +69,6 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act
 
     dz = dy act'(z) is rounded to the operands' type (as dy is where it is fp32) because the tensor cores take it as an operand;
     dbias sums it before that rounding, in fp32 and in a fixed order."""
-    from . import api
     act = _activation(activation)
     bias_dtype = x.dtype if bias_dtype is None else bias_dtype
     if bias_dtype != x.dtype and bias_dtype != torch.float32:

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, api
 
 
 def _stream(t: torch.Tensor):
@@ -173,7 +173,6 @@ def combine_topk_backward(dy: torch.Tensor, rows: torch.Tensor, pos: Optional[to
     dweights[t, j] = <dy[t], rows[pos]> in fp32; drows[pos] = weights[t, j] * dy[t], rounded once, and 0 in rows that no
     slot names. Slots with a pos outside the rows add nothing. With `need_rows` a row may be named by one slot only, as every
     layout here does: a second one sets the status word (`check_status` raises). cols must be a multiple of 8."""
-    from . import api
     w = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.to(torch.float32).contiguous()
     return _lib.torch_ops().combine_topk_backward(dy, rows, pos, w, bool(need_rows), bool(need_weights), api._status_word(dy.device))
 
@@ -280,12 +279,10 @@ def route_layout(topk_ids: torch.Tensor, num_experts: int, alignment: int = 128)
     `alignment` rows. `row_token` has room for the worst case (all pairs plus one alignment per expert), -1 past the last row.
     Ids of -1 (no expert) get no row; other ids outside [0, num_experts) do neither and set the status word (`check_status`
     raises). At most 1024 experts."""
-    from . import api
     return RouteLayout(*_lib.torch_ops().route_layout(topk_ids, int(num_experts), int(alignment), api._status_word(topk_ids.device)))
 
 
 def route_layout_masked(topk_ids: torch.Tensor, num_experts: int, max_rows: int) -> MaskedRouteLayout:
     """As `route_layout` for the masked layout: expert e has the rows e * max_rows ... of [num_experts, max_rows]. Pairs that find
     their expert's rows taken are dropped (row -1; first come, first served in token order), as a router with a capacity does."""
-    from . import api
     return MaskedRouteLayout(*_lib.torch_ops().route_layout_masked(topk_ids, int(num_experts), int(max_rows), api._status_word(topk_ids.device)))
