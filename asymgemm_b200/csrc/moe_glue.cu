@@ -255,7 +255,14 @@ __global__ void __launch_bounds__(256) combine_topk_f32_kernel(const float* __re
 // chunks of 8, whose loads are independent of each other (8 x 16 bytes in flight per thread). 4096 x 7168, top 8, bf16: 953 MB in
 // 192 us (5.0 TB/s); with streaming cache hints 274.
 //   dweights[t, j] = <dy[t], rows[pos]> (fp32, threads' parts joined in a fixed order), drows[pos] = w[t, j] * dy[t].
-constexpr int kGradThreads = 128;
+// Rows that no pair names (padding of the layout) get zeros, and a second pair with the same row is reported. The pairs leave a flag
+// per row (row_seen, cleared before) for zero_unseen_rows_kernel: three launches. Small calls, which those bound, take one: its
+// first blocks (SCAN) each own a run of rows, look through all pairs for them and fill the rest with zeros. Tokens x top k,
+// rows of cols bf16, flags / scan: 64 x 2, 1152 of 4096: 11.2 / 6.5 us; 1000 x 4, 11776 of 2048: 19.0 / 18.5; 1000 x 8, 40832 of 2048:
+// 42.7 / 47.5 (the larger kernel's blocks write zeros at 4.5 TB/s); 4000 x 8, 40192 of 1024: 48 / 63 (reading the pairs).
+constexpr int kGradThreads = 128, kScanRows = 4096, kScanBlocks = 1184;      // blocks: 8 per SM
+constexpr long long kScanPairs = 4096, kScanBytes = 64ll << 20;      // most pairs, most bytes of rows
+static_assert(kScanBytes / 16 <= static_cast<long long>(kScanRows) * kScanBlocks, "a row has 16 bytes at least");
 
 __device__ __forceinline__ void unpack8(const __nv_bfloat16* src, float (&v)[8]) {
   const uint4 u = *reinterpret_cast<const uint4*>(src);
@@ -283,13 +290,52 @@ __device__ __forceinline__ void store8(float* dst, const float (&v)[8]) {
 }
 
 template <typename T>
+__device__ __forceinline__ void zero_row(T* row, int cols, int lane) {
+  const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int c = lane * 8; c < cols; c += 256) store8(row + c, zero);
+}
+
+// One block's run of rows first .. first + count - 1 (count <= kScanRows), seen by the whole block.
+template <typename T>
+__device__ __forceinline__ void scan_and_zero(const long long* pos, long long pairs, long long first, int count, int cols, T* drows, int* status) {
+  __shared__ unsigned named[kScanRows / 32];
+  for (int i = threadIdx.x; i < (count + 31) / 32; i += kGradThreads) named[i] = 0;
+  __syncthreads();
+  constexpr int U = 8;      // loads under way together
+  for (long long i0 = threadIdx.x; i0 < pairs; i0 += U * kGradThreads) {
+    long long at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * kGradThreads;
+      at[u] = i >= pairs ? -1 : pos != nullptr ? pos[i] : i;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] < first || at[u] >= first + count) continue;
+      const int r = static_cast<int>(at[u] - first);
+      const unsigned bit = 1u << (r & 31);
+      if ((atomicOr(&named[r >> 5], bit) & bit) != 0 && status != nullptr) atomicCAS(status, 0, AG_COMBINE_ROW_TWICE);
+    }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < count; r += kGradThreads / 32)
+    if ((named[r >> 5] >> (r & 31) & 1u) == 0) zero_row(drows + (first + r) * cols, cols, threadIdx.x & 31);
+}
+
+template <typename T, bool SCAN>
 __global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const __nv_bfloat16* __restrict__ dy, const T* __restrict__ rows, long long num_rows,
                                                                     const long long* __restrict__ pos, const float* __restrict__ w, int top_k, int cols,
                                                                     T* __restrict__ drows, float* __restrict__ dweights,
-                                                                    unsigned char* __restrict__ row_seen, int* __restrict__ status) {
+                                                                    unsigned char* __restrict__ row_seen, int* __restrict__ status,
+                                                                    long long tokens, int scan_rows, int scan_blocks) {
   constexpr int J = 8;
   __shared__ float part[kGradThreads / 32][J];
-  const long long t = blockIdx.x;
+  if (SCAN && static_cast<int>(blockIdx.x) < scan_blocks) {
+    const long long first = static_cast<long long>(blockIdx.x) * scan_rows;
+    scan_and_zero(pos, tokens * top_k, first, static_cast<int>(min(static_cast<long long>(scan_rows), num_rows - first)), cols, drows, status);
+    return;
+  }
+  const long long t = SCAN ? blockIdx.x - scan_blocks : blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int j0 = 0; j0 < top_k; j0 += J) {
     long long row[J];
@@ -305,7 +351,7 @@ __global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const __nv_b
         wt[j] = w[pair];
       }
     }
-    if (drows != nullptr && threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < top_k) {
+    if (!SCAN && drows != nullptr && threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < top_k) {
       const long long pair = t * top_k + j0 + threadIdx.x;
       const long long r = pos != nullptr ? pos[pair] : pair;
       if (r >= 0 && r < num_rows) {
@@ -358,14 +404,13 @@ __global__ void __launch_bounds__(kGradThreads) combine_grad_kernel(const __nv_b
   }
 }
 
-// Rows that no pair named (padding of the layout) have gradient 0. One warp per row; 5.9 TB/s of writes.
+// Zeros in the rows without a flag. One warp per row; 5.9 TB/s of writes.
 template <typename T>
 __global__ void __launch_bounds__(256) zero_unseen_rows_kernel(T* __restrict__ drows, const unsigned char* __restrict__ row_seen, long long num_rows,
                                                                int cols) {
   const long long r = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   if (r >= num_rows || row_seen[r] != 0) return;
-  const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int c = (threadIdx.x & 31) * 8; c < cols; c += 256) store8(drows + r * cols + c, zero);
+  zero_row(drows + r * cols, cols, threadIdx.x & 31);
 }
 
 }  // namespace agb
@@ -374,17 +419,27 @@ namespace {
 template <typename T>
 cudaError_t launch_combine_grad(const void* dy, const void* rows, long long num_rows, const long long* pos, const float* w, long long tokens, int top_k,
                                 int cols, void* drows, float* dweights, void* row_seen, int* status, cudaStream_t stream) {
+  const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(dy);
+  const T* x = static_cast<const T*>(rows);
+  T* dx = static_cast<T*>(drows);
+  if (drows != nullptr && tokens * top_k <= agb::kScanPairs && num_rows <= agb::kScanBytes / static_cast<int>(sizeof(T)) / cols) {
+    const long long least = (num_rows + agb::kScanBlocks - 1) / agb::kScanBlocks;
+    const int scan_rows = least > 16 ? static_cast<int>(least) : 16, scan_blocks = static_cast<int>((num_rows + scan_rows - 1) / scan_rows);
+    if (tokens + scan_blocks > 0)
+      agb::combine_grad_kernel<T, true><<<static_cast<unsigned>(tokens + scan_blocks), agb::kGradThreads, 0, stream>>>(
+          g, x, num_rows, pos, w, top_k, cols, dx, dweights, nullptr, status, tokens, scan_rows, scan_blocks);
+    return cudaGetLastError();
+  }
   if (drows != nullptr && num_rows > 0) {
     cudaError_t e = cudaMemsetAsync(row_seen, 0, static_cast<size_t>((num_rows + 3) / 4 * 4), stream);
     if (e != cudaSuccess) return e;
   }
   if (tokens > 0)
-    agb::combine_grad_kernel<T><<<static_cast<unsigned>(tokens), agb::kGradThreads, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(dy), static_cast<const T*>(rows), num_rows, pos, w, top_k, cols, static_cast<T*>(drows), dweights,
-        static_cast<unsigned char*>(row_seen), status);
+    agb::combine_grad_kernel<T, false><<<static_cast<unsigned>(tokens), agb::kGradThreads, 0, stream>>>(
+        g, x, num_rows, pos, w, top_k, cols, dx, dweights, static_cast<unsigned char*>(row_seen), status, tokens, 0, 0);
   if (drows != nullptr && num_rows > 0)
     agb::zero_unseen_rows_kernel<T><<<static_cast<unsigned>((num_rows + 7) / 8), 256, 0, stream>>>(
-        static_cast<T*>(drows), static_cast<const unsigned char*>(row_seen), num_rows, cols);
+        dx, static_cast<const unsigned char*>(row_seen), num_rows, cols);
   return cudaGetLastError();
 }
 int launch_check() {

@@ -426,6 +426,38 @@ def test_layers_record_no_gradient():
     assert moe_ops.combine_topk(out, state.tables.pair_row, w, 20, 2).requires_grad
 
 
+@pytest.mark.expects_status
+@pytest.mark.parametrize("tokens,k,cols,rows", [(1024, 4, 8, 5000), (1025, 4, 8, 5000), (3, 2, 8, 4194304), (3, 2, 8, 4194305), (700, 5, 8, 40001), (0, 3, 16, 77),
+                                                (16, 2, 16384, 2048), (16, 2, 16384, 2049)])
+def test_gradient_rows_with_and_without_flags(tokens, k, cols, rows):
+    """Both sides of the sizes at which the rows that no pair names are found another way, and a row named twice in each."""
+    gen = torch.Generator().manual_seed(rows)
+    pos = torch.randint(rows, (4 * tokens * k,), generator=gen).unique()
+    pos = pos[torch.randperm(pos.numel(), generator=gen)][: tokens * k]
+    if tokens:
+        pos[0], pos[1], pos[2] = rows, -1, rows - 1
+        pos[3:] = torch.where(pos[3:] == rows - 1, -7, pos[3:])
+    assert pos.numel() == tokens * k
+    x, w = torch.randn((rows, cols), device=DEV).to(torch.bfloat16), torch.rand((tokens, k), device=DEV)
+    dy = randn(tokens, cols, seed=39, dtype=torch.bfloat16, scale=1.0)
+    drows, dweights = moe_ops.combine_topk_backward(dy, x, pos.to(DEV), w)
+    live = ((pos >= 0) & (pos < rows)).to(DEV)
+    at = pos.to(DEV)[live]
+    want = torch.zeros((rows, cols), dtype=torch.float64, device=DEV)
+    want[at] = (w.double().view(-1, 1) * dy.double().repeat_interleave(k, 0))[live]
+    assert bool(((drows.double() - want).abs() <= want.abs() * (2 ** -8 + 2 ** -23)).all())
+    terms = torch.zeros((tokens * k, cols), dtype=torch.float64, device=DEV)
+    terms[live] = dy.double().repeat_interleave(k, 0)[live] * x[at].double()
+    steps = cols / 128 + 8 + 9      # as above
+    assert bool(((dweights.double().view(-1) - terms.sum(1)).abs() <= terms.abs().sum(1) * steps * 2 ** -24).all())
+    ag.check_status()
+    if tokens:
+        pos[-1] = rows - 1
+        moe_ops.combine_topk_backward(dy, x, pos.to(DEV), w)
+        with pytest.raises(RuntimeError, match="same row"):
+            ag.check_status()
+
+
 def test_gradient_of_the_combine_without_a_position_table():
     rows, w = randn(60, 256, seed=40, dtype=torch.bfloat16), torch.rand((20, 3), device=DEV)
     dy = randn(20, 256, seed=41, dtype=torch.bfloat16)
