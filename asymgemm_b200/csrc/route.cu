@@ -874,16 +874,16 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
 // A stable counting sort of the (token, slot) pairs by expert, on integers only: the same input gives the same tables.
 // Every block owns a run of consecutive pairs, every warp of it a run of those. How many pairs of an expert lie before
 // a warp's run follows from the blocks' counts (first kernel, or the one block's own) and the warps' counts (shared
-// memory); inside a warp 32 pairs are ranked at a time with match.any. 524288 pairs, 256 experts: 19 us for both kernels (moving
-// their 13 MB would take 2); 512 pairs: 11 us in the one. What takes the time is the chain of short passes with barriers between
-// them, not any resource: issue slots are 28 % used. A run per block of 4096 pairs keeps every pair in a register meanwhile.
+// memory); inside a warp 32 pairs are ranked at a time with match.any. 524288 pairs, 256 experts: 16 us for both kernels (moving
+// their 13 MB would take 2); 512 pairs: 6.6 us in the one. What takes the time is the chain of short passes with barriers between
+// them, not any resource: issue slots are 28 % used. Runs of up to 4096 pairs per block stay in registers, experts and ranks, between the passes.
 struct LayoutParams {
   const void* ids;
   int ids_64;
   long long pairs;
   int top_k, experts, alignment, max_rows;    // max_rows > 0: the masked layout
   long long rows;                             // rows of the layout = entries of row_token
-  int* block_counts;                          // [blocks, experts]
+  int* block_counts;                          // [blocks, experts rounded up to 4]
   long long* pair_row;
   long long* row_token;
   long long* rows_per_expert;                 // contiguous
@@ -896,6 +896,8 @@ struct LayoutParams {
 
 constexpr int kLayoutThreads = 1024;
 constexpr int kLayoutWarps = kLayoutThreads / 32;
+
+__host__ __device__ constexpr int padded_experts(int experts) { return (experts + 3) & ~3; }
 
 __device__ __forceinline__ int pair_expert(const LayoutParams& p, long long i, bool report) {
   const long long e = p.ids_64 ? __ldg(static_cast<const long long*>(p.ids) + i) : __ldg(static_cast<const int*>(p.ids) + i);
@@ -914,10 +916,11 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_count_kernel(const Layo
     if (e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) p.block_counts[static_cast<long long>(blockIdx.x) * p.experts + e] = count[e];
+  for (int e = threadIdx.x; e < p.experts; e += kLayoutThreads) p.block_counts[static_cast<long long>(blockIdx.x) * padded_experts(p.experts) + e] = count[e];
 }
 
-// ONE: the launch is a single block, which needs no counts of others.
+// ONE: the pairs are one block's, which needs no counts of others. The launch's further blocks, if any, count the same pairs and only
+// take part in marking the rows that none has.
 template <bool ONE>
 __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const LayoutParams p) {
   extern __shared__ int smem[];
@@ -932,54 +935,70 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
   for (int i = threadIdx.x; i < kLayoutWarps * E; i += kLayoutThreads) mine[i] = 0;
   __syncthreads();
 
-  const long long begin = blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
+  const long long begin = ONE ? 0 : blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
   const long long share = p.run / kLayoutWarps;            // a multiple of 32
   const long long from = begin + warp * share, to = min(from + share, end);
   // the warp's pairs, kept in registers 4 x 32 at a time so that their loads are under way together (a run of 4096 pairs per
-  // block is just that; a longer one is read again below)
+  // block is the most that stays; a longer one is read again below)
   constexpr int kAhead = 4;
   int mine_e[kAhead];
+  unsigned same_e[kAhead];      // lanes with the same expert
   auto load_pairs = [&](long long i0, bool report) {
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const long long i = i0 + 32 * q + lane;
       mine_e[q] = i < to ? pair_expert(p, i, report) : -1;
     }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) same_e[q] = __match_any_sync(kAll, mine_e[q]);
   };
   for (long long i0 = from; i0 < to; i0 += 32 * kAhead) {
-    load_pairs(i0, true);
+    load_pairs(i0, !ONE || blockIdx.x == 0);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const int e = mine_e[q];
-      const unsigned same = __match_any_sync(kAll, e);
+      const unsigned same = same_e[q];
       if (e >= 0 && lane == __ffs(same) - 1) mine[warp * E + e] += __popc(same);
       __syncwarp();
     }
   }
   if (!ONE) {
-    // all blocks' counts, `parts` threads per expert; integer sums, so their order does not matter
-    const int parts = max(1, kLayoutThreads / E);
-    for (int i = threadIdx.x; i < parts * E; i += kLayoutThreads) {
-      const int e = i % E;
-      int all = 0, before = 0;
+    // all blocks' counts, four experts at a time, `parts` threads for each four; integer sums, so their order does not matter
+    const int fours = padded_experts(E) / 4, parts = kLayoutThreads / fours;
+    const int part = static_cast<int>(threadIdx.x) / fours, e0 = static_cast<int>(threadIdx.x) % fours * 4;
+    if (part < parts) {
+      int all[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0};
 #pragma unroll 8
-      for (int b = i / E; b < static_cast<int>(gridDim.x); b += parts) {
-        const int v = __ldg(p.block_counts + static_cast<long long>(b) * E + e);
-        all += v;
-        before += b < static_cast<int>(blockIdx.x) ? v : 0;
+      for (int b = part; b < static_cast<int>(gridDim.x); b += parts) {
+        const int4 v = __ldg(reinterpret_cast<const int4*>(p.block_counts) + static_cast<long long>(b) * fours + e0 / 4);
+        const int c[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          all[j] += c[j];
+          before[j] += b < static_cast<int>(blockIdx.x) ? c[j] : 0;
+        }
       }
-      atomicAdd(&total[e], all);
-      atomicAdd(&seen[e], before);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (e0 + j >= E) break;      // what the padding holds is not used
+        atomicAdd(&total[e0 + j], all[j]);
+        atomicAdd(&seen[e0 + j], before[j]);
+      }
     }
   }
   __syncthreads();
   // pairs of the expert before each warp's run, in this block
   for (int e = threadIdx.x; e < E; e += kLayoutThreads) {
     int before = seen[e];
-    for (int w = 0; w < kLayoutWarps; ++w) {
-      const int v = mine[w * E + e];
-      mine[w * E + e] = before;
-      before += v;
+    for (int w0 = 0; w0 < kLayoutWarps; w0 += 8) {
+      int v[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v[w] = mine[(w0 + w) * E + e];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        mine[(w0 + w) * E + e] = before;
+        before += v[w];
+      }
     }
     if (ONE) total[e] = before;
   }
@@ -1025,13 +1044,13 @@ __global__ void __launch_bounds__(kLayoutThreads) layout_place_kernel(const Layo
     }
     __syncthreads();
   }
-  for (long long i0 = from; i0 < to; i0 += 32 * kAhead) {
+  for (long long i0 = from; i0 < to && (!ONE || blockIdx.x == 0); i0 += 32 * kAhead) {
     if (to - from > 32 * kAhead) load_pairs(i0, false);
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const long long i = i0 + 32 * q + lane;
       const int e = mine_e[q];
-      const unsigned same = __match_any_sync(kAll, e);
+      const unsigned same = same_e[q];
       int base = 0;
       if (e >= 0) base = mine[warp * E + e];
       __syncwarp();
@@ -1125,11 +1144,14 @@ void launch_route_backward(const agb::RouteGradParams& p, bool vector, cudaStrea
   else agb::route_topk_backward_kernel<T, false><<<grid, 128, 0, stream>>>(p);
 }
 
-// Pairs per block: 4096 keep one block for a decode batch, and no more than 128 blocks, because every block sums the
-// counts of all others.
+// Pairs per block. Up to 2048 one block saves the counting launch (256 experts: 2048 pairs 8.4 us in one, 10.7 in two; 4096 pairs 12.1
+// and 9.8). Then runs of 1024, one pair per thread (32768 pairs: 9.6 us; in runs of 2048 11.5, of 4096 15.1), but no more than 128
+// blocks, because every block sums the counts of all others (524288 pairs: 16 us on 128 blocks, 23 on 256).
+constexpr int64_t kLayoutFill = 4096, kLayoutRun = 1024;
 long long layout_run(long long pairs) {
+  if (pairs <= 2048) return 2048;
   const long long run = (pairs + 127) / 128;
-  const long long least = run > 4096 ? run : 4096;
+  const long long least = run > kLayoutRun ? run : kLayoutRun;
   return (least + agb::kLayoutThreads - 1) / agb::kLayoutThreads * agb::kLayoutThreads;
 }
 
@@ -1220,7 +1242,7 @@ int ag_route_topk_backward(const void* logits, int32_t dtype, int64_t tokens, in
 uint64_t ag_route_layout_workspace_bytes(int64_t pairs, int32_t experts) {
   if (pairs <= 0 || experts <= 0) return 0;
   const int64_t blocks = (pairs + layout_run(pairs) - 1) / layout_run(pairs);
-  return blocks > 1 ? static_cast<uint64_t>(blocks) * experts * 4 : 0;
+  return blocks > 1 ? static_cast<uint64_t>(blocks) * agb::padded_experts(experts) * 4 : 0;
 }
 
 int ag_route_layout(const ag_route_layout_desc_t* r) {
@@ -1230,8 +1252,8 @@ int ag_route_layout(const ag_route_layout_desc_t* r) {
   const int64_t pairs = r->tokens * r->top_k;
   if (pairs > 0x7fffffffLL / 2 || r->rows > 0x7fffffffLL) return agb_fail(AG_E_INVALID, "too many (token, slot) pairs");
   if (!aligned_to(r->ids, r->ids_64 ? 8 : 4) || !aligned_to(r->pair_row, 8) || !aligned_to(r->row_token, 8) || !aligned_to(r->rows_per_expert, 8) ||
-      !aligned_to(r->offsets, 4) || !aligned_to(r->expert_list, 4) || !aligned_to(r->masked_m, 4) || !aligned_to(r->workspace, 4))
-    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type");
+      !aligned_to(r->offsets, 4) || !aligned_to(r->expert_list, 4) || !aligned_to(r->masked_m, 4) || !aligned_to(r->workspace, 16))
+    return agb_fail(AG_E_INVALID, "pointers must be aligned to their element type, the workspace to 16 bytes");
   if ((pairs > 0 && (r->ids == nullptr || r->pair_row == nullptr)) || (r->rows > 0 && r->row_token == nullptr))
     return agb_fail(AG_E_INVALID, "ids, pair_row and row_token must be non-NULL");
   if (r->max_rows > 0) {
@@ -1274,7 +1296,10 @@ int ag_route_layout(const ag_route_layout_desc_t* r) {
     if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   }
   if (blocks > 1) agb::layout_count_kernel<<<blocks, agb::kLayoutThreads, static_cast<size_t>(r->experts) * 4, stream>>>(p);
-  place<<<blocks, agb::kLayoutThreads, smem, stream>>>(p);
+  // few pairs: a block more for every kLayoutFill rows to be marked (64 pairs x 8, 256 experts, 33280 rows: 10.5 us on one block, 6.6 on 9)
+  const int64_t fill = (r->rows + kLayoutFill - 1) / kLayoutFill;
+  const int grid = blocks > 1 ? blocks : fill < 1 ? 1 : fill > 64 ? 64 : static_cast<int>(fill);
+  place<<<grid, agb::kLayoutThreads, smem, stream>>>(p);
   return launch_check();
 }
 

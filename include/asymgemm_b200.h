@@ -393,7 +393,7 @@ typedef struct ag_route_layout_desc {
   int32_t* offsets;
   int32_t* expert_list;
   int32_t* masked_m;
-  void* workspace;         /* ag_route_layout_workspace_bytes(tokens * top_k, experts) bytes, this call's alone while it runs */
+  void* workspace;         /* ag_route_layout_workspace_bytes(tokens * top_k, experts) bytes, 16-byte aligned, this call's alone while it runs */
   uint64_t workspace_bytes;
   int32_t* status;
   void* stream;

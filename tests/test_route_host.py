@@ -61,7 +61,7 @@ def test_layout_refuses_bad_descriptors():
         assert lib.ag_route_layout(layout_desc(**bad)) == BAD, bad
     for tokens in (1 << 62, (1 << 63) - 1):      # tokens * top_k does not fit in 64 bits
         assert lib.ag_route_layout(layout_desc(tokens=tokens)) == BAD
-    assert lib.ag_route_layout_workspace_bytes(4096, 256) == 0 and lib.ag_route_layout_workspace_bytes(4097, 256) == 2 * 256 * 4
+    assert lib.ag_route_layout_workspace_bytes(2048, 256) == 0 and lib.ag_route_layout_workspace_bytes(2049, 254) == 3 * 256 * 4
     assert lib.ag_route_layout_workspace_bytes(0, 8) == 0 and lib.ag_route_layout_workspace_bytes(-5, 8) == 0
 
 
