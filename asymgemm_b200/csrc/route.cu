@@ -876,7 +876,7 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
 // a warp's run follows from the blocks' counts (first kernel, or the one block's own) and the warps' counts (shared
 // memory); inside a warp 32 pairs are ranked at a time with match.any. 524288 pairs, 256 experts: 16 us for both kernels (moving
 // their 13 MB would take 2); 512 pairs: 6.6 us in the one. What takes the time is the chain of short passes with barriers between
-// them, not any resource: issue slots are 28 % used. Runs of up to 4096 pairs per block stay in registers, experts and ranks, between the passes.
+// them, not any resource: issue slots are 29 % used. Runs of up to 4096 pairs per block stay in registers, experts and ranks, between the passes.
 struct LayoutParams {
   const void* ids;
   int ids_64;
