@@ -320,6 +320,26 @@ def test_contiguous_layout(tokens, experts, k, dtype):
         assert got.experts.tolist() == list(range(experts)) + [-1] and got.experts.dtype == torch.int32
 
 
+@pytest.mark.parametrize("tokens,experts,k", [(256, 256, 8), (2048, 16, 1), (2049, 16, 1), (150001, 7, 4), (131073, 60, 4), (700000, 3, 1)])
+def test_layouts_on_either_side_of_their_block_sizes(tokens, experts, k):
+    """One block, several, and so many pairs that a block's do not stay in registers; every table of both layouts."""
+    ids = make_ids(tokens, experts, k, tokens + experts, 0.1).to(DEV)
+    got = moe_ops.route_layout(ids, experts)
+    pair_row, row_token, count, offsets, _ = plain_layout(ids, experts, got.row_token.numel())
+    assert torch.equal(got.pair_row.cpu(), pair_row) and torch.equal(got.row_token.cpu(), row_token)
+    assert torch.equal(got.rows_per_expert.cpu(), count) and torch.equal(got.offsets.cpu(), offsets)
+    max_rows = tokens * k // experts
+    masked = moe_ops.route_layout_masked(ids, experts, max_rows)
+    # the same order within an expert, its rows elsewhere and no more than max_rows of them
+    flat = ids.view(-1).cpu()
+    within = pair_row - offsets.view(-1, 2)[flat.clamp(min=0), 0]
+    want = torch.where((flat >= 0) & (within < max_rows), flat * max_rows + within, -1)
+    assert torch.equal(masked.pair_row.cpu(), want) and torch.equal(masked.masked_m.cpu().long(), count.clamp(max=max_rows))
+    tokens_of = torch.full((experts * max_rows,), -1, dtype=torch.int64)
+    tokens_of[want[want >= 0]] = (torch.arange(tokens * k) // k)[want >= 0]
+    assert torch.equal(masked.row_token.cpu(), tokens_of)
+
+
 @pytest.mark.parametrize("tokens,experts,k,max_rows", [(0, 3, 2, 4), (1, 8, 2, 1), (64, 256, 8, 16), (100, 8, 4, 30), (4000, 16, 4, 600), (2000, 4, 2, 1500)])
 def test_masked_layout_drops_what_does_not_fit(tokens, experts, k, max_rows):
     for missing in (0.0, 0.2):
