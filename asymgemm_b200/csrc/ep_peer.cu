@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) ep_histogram_kernel(const long long* __re
   for (long long p = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; p < pairs; p += static_cast<long long>(gridDim.x) * blockDim.x) {
     const long long e = ids[p];
     if (e >= 0 && e < num_experts) atomicAdd(&hist[e], 1);
-    else atomicCAS(status, 0, AG_EP_BAD_EXPERT);
+    else if (e != -1) atomicCAS(status, 0, AG_EP_BAD_EXPERT);      // -1: the pair has no expert
   }
   __syncthreads();
   for (int i = threadIdx.x; i < num_experts; i += blockDim.x)
@@ -139,7 +139,9 @@ __device__ __forceinline__ int owner_of(const int* range_lo, int world, int e) {
 
 // One warp per (token, slot) pair p: the token's quantised row, its scales and the pair's return address go to the next
 // free row of its expert on the owner rank. Rows of one expert land in no particular order; every row's result is
-// independent of its position, so the layer's output does not depend on that order.
+// independent of its position, so the layer's output does not depend on that order. A pair without an expert (id -1, as the
+// router marks padding tokens, or outside the experts, which the histogram reports) goes nowhere, and neither does one for
+// which the owner has no room left (the plan reports that): their pair_row is -1, so that the combine leaves them out.
 __global__ void __launch_bounds__(256) ep_dispatch_kernel(const uint4* __restrict__ x_q, const float* __restrict__ sfx,
                                                           const long long* __restrict__ ids, long long pairs, int top_k, int vec_per_row,
                                                           int sf_per_row, const int* __restrict__ range_lo, int world, int me,
@@ -151,14 +153,20 @@ __global__ void __launch_bounds__(256) ep_dispatch_kernel(const uint4* __restric
   const long long p = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (p >= pairs) return;
-  const int e = static_cast<int>(ids[p]);
+  const long long id = ids[p];
+  const bool routed = id >= 0 && id < lo[world];      // the ranks' ranges end with the last expert
+  const int e = routed ? static_cast<int>(id) : 0;
+  long long dest = -1;
+  if (routed) {
+    int slot = 0;
+    if (lane == 0) slot = atomicAdd(&cursors[e], 1);
+    slot = __shfl_sync(0xffffffffu, slot, 0);
+    dest = static_cast<long long>(send_base[e]) + slot;
+    if (dest >= cap_rows) dest = -1;
+  }
+  if (pair_row != nullptr && lane == 0) pair_row[p] = dest;
+  if (dest < 0) return;
   const int o = owner_of(lo, world, e);
-  int slot = 0;
-  if (lane == 0) slot = atomicAdd(&cursors[e], 1);
-  slot = __shfl_sync(0xffffffffu, slot, 0);
-  const long long dest = static_cast<long long>(send_base[e]) + slot;
-  if (pair_row != nullptr && lane == 0) pair_row[p] = dest < cap_rows ? dest : 0;   // one rank: where this pair's result will be
-  if (dest >= cap_rows) return;   // the plan kernel has flagged the overflow
   const long long t = p / top_k;
   const uint4* src = x_q + t * vec_per_row;
   uint4* dst = static_cast<uint4*>(peers.a[o]) + dest * vec_per_row;

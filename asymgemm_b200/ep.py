@@ -570,13 +570,13 @@ class ExpertParallelMoE:
         self._mark("layout")
         # more than one rank: the down GEMM's drain stores every result row straight into its pair's slot of the source rank's
         # combine buffer (over NVLink, tile by tile while the GEMM runs); there is no separate return pass
-        direct = px.pair_row is None and self.fused_return
+        direct = px.world > 1 and self.fused_return
         out = self.experts_forward(a_q, px.sfa, state, rows_used=px.rows_used[:1], scatter=(px.meta, px.ret_bases) if direct else None)
         if self.prefetch_next is not None and out.is_cuda:      # staged weight path: start the next call's first copies now
             api.prefetch_weights(self.prefetch_next, out.device)
-        if px.pair_row is not None:      # one rank: every result already lies in this rank's memory
+        if px.world == 1:      # every result already lies in this rank's memory
             self._mark("return")
-            y = moe_ops.combine_topk_forward(out, px.pair_row, topk_weights, tokens, top_k)
+            y = moe_ops.combine_topk_forward(out, px.result_rows(), topk_weights, tokens, top_k)
             self._mark("combine")
             return y
         if direct:
@@ -584,7 +584,7 @@ class ExpertParallelMoE:
         else:
             px.send_back(out)
         self._mark("return")
-        y = moe_ops.combine_topk_forward(px.ret.view(torch.bfloat16).view(px.pairs_cap, self.hidden), None, topk_weights, tokens, top_k)
+        y = moe_ops.combine_topk_forward(px.ret.view(torch.bfloat16).view(px.pairs_cap, self.hidden), px.result_rows(), topk_weights, tokens, top_k)
         self._mark("combine")
         return y
 

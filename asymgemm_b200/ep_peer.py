@@ -126,8 +126,9 @@ class PeerExchange:
         self.experts = torch.full((self.epr + 1,), -1, dtype=torch.int32, device=device)
         self.rows_used = torch.zeros(2, dtype=torch.int32, device=device)
         self._token = torch.zeros(1, dtype=torch.int32, device=device)
-        # one rank: row of every pair in the layout, so that the results are combined where they lie (no return copy)
-        self.pair_row = torch.zeros(pairs, dtype=torch.int64, device=device) if self.world == 1 else None
+        # row of every pair in its owner's layout, -1 = sent nowhere. One rank: the results are combined where they lie (no return copy)
+        self.pair_row = torch.full((pairs,), -1, dtype=torch.int64, device=device)
+        self._slots = torch.arange(pairs, device=device) if self.world > 1 else None
         torch.cuda.synchronize(device)
         if self.world > 1:
             dist.barrier(group=group)      # every rank has mapped every buffer before anyone stores into one
@@ -172,10 +173,16 @@ class PeerExchange:
         with torch.cuda.device(self.device):
             _lib.check(lib.ag_ep_dispatch(x_q.data_ptr(), sfx.data_ptr(), self._ids.data_ptr(), tokens, self.top_k, self.row_bytes,
                                           self.sf_per_row, self.range_lo.data_ptr(), self.world, self.rank, self.send_base.data_ptr(),
-                                          self.cursors.data_ptr(), self.cap_rows,
-                                          self.pair_row.data_ptr() if self.pair_row is not None else None,
+                                          self.cursors.data_ptr(), self.cap_rows, self.pair_row.data_ptr(),
                                           ctypes.byref(self.peers), self._stream()))
         self.rendezvous()
+
+    def result_rows(self) -> torch.Tensor:
+        """Where the result of every pair of the last `dispatch` will be, -1 for pairs that were sent nowhere (`pos` of
+        `moe_ops.combine_topk`): rows of this rank's layout (one rank), or the pairs' own slots of `ret`, of which nobody writes
+        those of the others in this step."""
+        went = self.pair_row[: self._ids.numel()]
+        return went if self.world == 1 else torch.where(went < 0, went, self._slots[: went.numel()])
 
     def send_back(self, out: torch.Tensor) -> None:
         """Store every valid row of `out` [cap_rows, *] (this rank's layout) into its pair's slot on the source rank."""

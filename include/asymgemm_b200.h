@@ -309,7 +309,8 @@ int ag_peer_open(const unsigned char* handle64, void** ptr);
 int ag_peer_close(void* ptr);
 int ag_peer_free(void* ptr);
 
-/* counts[e] = (token, slot) pairs of ids [pairs] (int64) routed to expert e; counts is zeroed first. */
+/* counts[e] = (token, slot) pairs of ids [pairs] (int64) routed to expert e; counts is zeroed first. Ids of -1 (no expert) count
+ * nowhere; other ids outside [0, num_experts) do neither and set the status word. */
 int ag_ep_histogram(const int64_t* ids, int64_t pairs, int32_t num_experts, int32_t* counts, int32_t* status, void* stream);
 
 /* From every rank's histogram counts_all [world, num_experts] and the ownership table range_lo [world + 1] (rank r owns
@@ -324,7 +325,9 @@ int ag_ep_plan(const int32_t* counts_all, const int32_t* range_lo, int32_t world
 /* Every (token, slot) pair of this rank: the token's row x_q [tokens, row_bytes] and scales sfx [tokens, sf_per_row] are
  * stored into the next free row of the pair's expert on the owner rank, with the pair's return address beside it.
  * pair_row (optional, int64 [tokens * top_k]) receives the row each pair went to: with one rank the results can then be
- * combined straight out of the layout (ag_combine_topk with pos = pair_row) and ag_ep_return is not needed. */
+ * combined straight out of the layout (ag_combine_topk with pos = pair_row) and ag_ep_return is not needed. Pairs with an id
+ * outside the experts, and pairs for which their owner has no room, are sent nowhere: their pair_row is -1 and nobody writes their
+ * slot of `ret`, so with several ranks combine with pos = the pair's own index, or -1 where pair_row is. */
 int ag_ep_dispatch(const void* x_q, const float* sfx, const int64_t* ids, int64_t tokens, int32_t top_k, int64_t row_bytes, int32_t sf_per_row,
                    const int32_t* range_lo, int32_t world, int32_t rank, const int32_t* send_base, int32_t* cursors, int64_t cap_rows,
                    int64_t* pair_row, const ag_ep_peers_t* peers, void* stream);
