@@ -84,6 +84,11 @@ def _row_bytes(t: torch.Tensor) -> int:
     return n
 
 
+def _never_empty(rows: torch.Tensor) -> torch.Tensor:
+    """`rows`, or one row of zeros where there are none: a table of nothing but -1 (an empty batch in the masked layout) reads none."""
+    return rows if rows.shape[0] else torch.cat([rows, rows.new_zeros((1,) + tuple(rows.shape[1:]))])
+
+
 def move_rows(src: torch.Tensor, out_rows: int, src_rows: Optional[torch.Tensor] = None, dst_rows: Optional[torch.Tensor] = None,
               count: Optional[int] = None, zero: bool = False) -> torch.Tensor:
     """out[dst_rows[i] or i] = src[src_rows[i] or i] for i < count. `out` has `out_rows` rows of src's row shape and dtype.
@@ -93,6 +98,8 @@ def move_rows(src: torch.Tensor, out_rows: int, src_rows: Optional[torch.Tensor]
     out = (torch.zeros if zero else torch.empty)((out_rows,) + tuple(src.shape[1:]), dtype=src.dtype, device=src.device)
     if count == 0:
         return out
+    if src_rows is not None:
+        src = _never_empty(src)
     rb = _row_bytes(src)
     if src.is_cuda and rb % 16 == 0 and src.is_contiguous():
         with torch.cuda.device(src.device):
@@ -145,6 +152,8 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
     cols = rows.shape[1]
     if tokens == 0:
         return torch.empty((0, cols), dtype=torch.bfloat16 if rows.is_cuda else rows.dtype, device=rows.device)
+    if pos is not None:
+        rows = _never_empty(rows)
     if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():
         y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
         w = weights.to(torch.float32).contiguous()
