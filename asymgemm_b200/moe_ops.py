@@ -95,31 +95,38 @@ def move_rows(src: torch.Tensor, out_rows: int, src_rows: Optional[torch.Tensor]
     A negative src_rows[i] writes a row of zeros, a negative dst_rows[i] writes nothing."""
     count = int(count if count is not None else (src_rows.numel() if src_rows is not None else
                                                  (dst_rows.numel() if dst_rows is not None else src.shape[0])))
-    out = (torch.zeros if zero else torch.empty)((out_rows,) + tuple(src.shape[1:]), dtype=src.dtype, device=src.device)
+
+    def room(rows):
+        return (torch.zeros if zero else torch.empty)((rows,) + tuple(src.shape[1:]), dtype=src.dtype, device=src.device)
+
     if count == 0:
-        return out
+        return room(out_rows)
     if src_rows is not None:
         src = _never_empty(src)
     rb = _row_bytes(src)
     if src.is_cuda and rb % 16 == 0 and src.is_contiguous():
+        out = room(out_rows)
         with torch.cuda.device(src.device):
             _lib.check(_lib.load().ag_move_rows(src.data_ptr(), out.data_ptr(),
                                                 src_rows.data_ptr() if src_rows is not None else None,
                                                 dst_rows.data_ptr() if dst_rows is not None else None, count, rb, _stream(src)))
         return out
+    # plain torch, without waiting for the device: rows without a destination go to one row more, behind the result
     s = src.view(torch.uint8) if src.dtype == torch.float8_e4m3fn else src
-    o = out.view(torch.uint8) if out.dtype == torch.float8_e4m3fn else out
     if src_rows is not None:
+        src_rows = src_rows[:count]
         picked = s.index_select(0, src_rows.clamp(min=0))
         picked.masked_fill_((src_rows < 0).view((-1,) + (1,) * (s.dim() - 1)), 0)
     else:
         picked = s[:count]
-    if dst_rows is not None:
-        keep = dst_rows >= 0
-        o.index_copy_(0, dst_rows[keep], picked[keep])
-    else:
+    out = room(out_rows + (dst_rows is not None))
+    o = out.view(torch.uint8) if out.dtype == torch.float8_e4m3fn else out
+    if dst_rows is None:
         o[:count] = picked
-    return out
+        return out
+    dst_rows = dst_rows[:count]
+    o.index_copy_(0, torch.where(dst_rows < 0, out_rows, dst_rows), picked)
+    return out[:out_rows]
 
 
 def move_rows_into(out: torch.Tensor, src: torch.Tensor, dst_rows: torch.Tensor) -> None:

@@ -25,3 +25,26 @@ def test_an_empty_batch_in_the_masked_layout(cols, dtype):
     assert out.shape == (32, cols) and float(out.float().abs().max()) == 0
     y = moe_ops.combine_topk(x, torch.full((6,), -1, device=DEV), torch.ones((3, 2), device=DEV), 3, 2)
     assert y.shape == (3, cols) and float(y.float().abs().max()) == 0
+
+
+@pytest.mark.parametrize("cols,dtype", [(5, torch.float32), (18, torch.float32), (12, torch.bfloat16), (40, torch.float8_e4m3fn), (64, torch.bfloat16)])
+def test_row_moves_without_a_kernel_do_not_wait_for_the_device(cols, dtype):
+    """Rows whose bytes are no multiple of 16 (scale rows of some widths): a call that waited could not be captured."""
+    src = randn(50, cols, seed=1).to(dtype)
+    gen = torch.Generator().manual_seed(2)
+    dst = torch.randperm(60, generator=gen)[:50]
+    dst[::7] = -1
+    pick = torch.randint(-1, 50, (50,), generator=gen)
+    dst, pick = dst.to(DEV), pick.to(DEV)
+    moe_ops.move_rows(src, 60, src_rows=pick, dst_rows=dst, zero=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = moe_ops.move_rows(src, 60, src_rows=pick, dst_rows=dst, zero=True)
+    src.copy_(randn(50, cols, seed=3).to(dtype))
+    graph.replay()
+    want = torch.zeros((60, cols), dtype=torch.float64)
+    for i, (d, s) in enumerate(zip(dst.tolist(), pick.tolist())):
+        if d >= 0 and s >= 0:
+            want[d] = src[s].cpu().double()
+    assert out.shape == (60, cols) and out.dtype == dtype and torch.equal(out.float().cpu().double(), want)

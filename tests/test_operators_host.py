@@ -28,3 +28,17 @@ def test_tables_of_missing_rows_read_nothing_where_there_are_no_rows(dtype):
         y = moe_ops.combine_topk(leaf, none, torch.ones(3, 2), 3, 2)
         assert y.shape == (3, 16) and y.dtype == dtype and float(y.detach().abs().max()) == 0
         assert torch.autograd.grad(y.sum(), leaf)[0].shape == (0, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float8_e4m3fn])
+def test_cpu_row_moves_with_and_without_a_destination(dtype):
+    src = torch.arange(30, dtype=torch.float32).view(6, 5).to(dtype)
+    dst = torch.tensor([2, -1, 0, -5, 3, 9])
+    out = moe_ops.move_rows(src, 4, dst_rows=dst, count=5, zero=True)
+    want = torch.stack([src[2], torch.zeros(5).to(dtype), src[0], src[4]])
+    assert out.shape == (4, 5) and out.dtype == dtype and torch.equal(out.float(), want.float())
+    out = moe_ops.move_rows(src, 4, src_rows=torch.tensor([5, -1, 1, 0, 3, 3]), dst_rows=dst, count=5, zero=True)
+    want = torch.stack([src[1], torch.zeros(5).to(dtype), src[5], src[3]])
+    assert torch.equal(out.float(), want.float())
+    out = moe_ops.move_rows(src, 4, src_rows=torch.tensor([5, -1, 1]), count=2, zero=True)
+    assert torch.equal(out[0].float(), src[5].float()) and float(out[1:].float().abs().max()) == 0
