@@ -142,13 +142,16 @@ def move_rows_into(out: torch.Tensor, src: torch.Tensor, dst_rows: torch.Tensor)
     out.index_copy_(0, dst_rows, src)
 
 
+def _has_combine_kernel(rows: torch.Tensor) -> bool:
+    return rows.is_cuda and rows.is_contiguous() and rows.shape[1] % {torch.bfloat16: 8, torch.float32: 4}.get(rows.dtype, 1 << 62) == 0
+
+
 def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
-    """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (CUDA: bf16); pos None =
-    t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
+    """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (bf16 where a CUDA kernel runs); pos
+    None = t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
     `weights`; where the CUDA kernels run (contiguous rows, bf16 with cols a multiple of 8 or fp32 with a multiple of 4) the
     gradient is `combine_topk_backward`'s: no two slots may name the same row, and cols must be a multiple of 8."""
-    kernel = rows.is_cuda and rows.is_contiguous() and rows.shape[1] % {torch.bfloat16: 8, torch.float32: 4}.get(rows.dtype, 1 << 62) == 0
-    if kernel and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if _has_combine_kernel(rows) and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
     return combine_topk_forward(rows, pos, weights, tokens, top_k)
 
@@ -158,7 +161,7 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
     either and whose buffers the next call overwrites."""
     cols = rows.shape[1]
     if tokens == 0:
-        return torch.empty((0, cols), dtype=torch.bfloat16 if rows.is_cuda else rows.dtype, device=rows.device)
+        return torch.empty((0, cols), dtype=torch.bfloat16 if _has_combine_kernel(rows) else rows.dtype, device=rows.device)
     if pos is not None:
         rows = _never_empty(rows)
     if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():

@@ -48,3 +48,11 @@ def test_row_moves_without_a_kernel_do_not_wait_for_the_device(cols, dtype):
         if d >= 0 and s >= 0:
             want[d] = src[s].cpu().double()
     assert out.shape == (60, cols) and out.dtype == dtype and torch.equal(out.float().cpu().double(), want)
+
+
+@pytest.mark.parametrize("dtype,cols", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float32, 12), (torch.float16, 64), (torch.bfloat16, 12), (torch.float32, 5)])
+def test_the_combine_of_an_empty_batch_has_the_type_of_any_other(dtype, cols):
+    rows, pos, w = randn(8, cols, seed=4, dtype=dtype), torch.arange(8, device=DEV), torch.rand((4, 2), device=DEV)
+    for fn in (moe_ops.combine_topk, moe_ops.combine_topk_forward):
+        full, empty = fn(rows, pos, w, 4, 2), fn(rows, pos[:0], w[:0], 0, 2)
+        assert empty.shape == (0, cols) and empty.dtype == full.dtype
