@@ -179,9 +179,11 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
                                                        _stream(rows)))
         return y
     picked = (rows.index_select(0, pos.clamp(min=0)) if pos is not None else rows[: tokens * top_k]).view(tokens, top_k, cols).float()
-    if pos is not None:
-        picked = torch.where((pos < 0).view(tokens, top_k, 1), picked.new_zeros(()), picked)
-    return (picked * weights.unsqueeze(-1).float()).sum(dim=1).to(rows.dtype)
+    w = weights.reshape(tokens, top_k, 1).float()
+    if pos is not None:      # what has no row adds nothing, whatever its weight and row 0 are
+        none = (pos < 0).view(tokens, top_k, 1)
+        picked, w = picked.masked_fill(none, 0), w.masked_fill(none, 0)
+    return (picked * w).sum(dim=1).to(rows.dtype)
 
 
 def combine_topk_backward(dy: torch.Tensor, rows: torch.Tensor, pos: Optional[torch.Tensor], weights: torch.Tensor, need_rows: bool = True,

@@ -42,3 +42,14 @@ def test_cpu_row_moves_with_and_without_a_destination(dtype):
     assert torch.equal(out.float(), want.float())
     out = moe_ops.move_rows(src, 4, src_rows=torch.tensor([5, -1, 1]), count=2, zero=True)
     assert torch.equal(out[0].float(), src[5].float()) and float(out[1:].float().abs().max()) == 0
+
+
+def test_cpu_combine_does_not_look_at_the_weight_of_a_missing_row():
+    rows = torch.arange(12.0).view(4, 3)
+    rows[0] = float("inf")
+    a, w = rows.requires_grad_(True), torch.tensor([[0.5, float("nan")], [float("inf"), 2.0]], requires_grad=True)
+    y = moe_ops.combine_topk(a, torch.tensor([1, -1, -1, 3]), w, 2, 2)
+    assert torch.equal(y, torch.stack([0.5 * rows[1], 2 * rows[3]]))
+    da, dw = torch.autograd.grad(y, (a, w), torch.ones(2, 3))
+    assert da.tolist() == [[0.0] * 3, [0.5] * 3, [0.0] * 3, [2.0] * 3]
+    assert dw.tolist() == [[float(rows[1].sum()), 0.0], [0.0, float(rows[3].sum())]]
