@@ -163,7 +163,7 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
     if tokens == 0:
         return torch.empty((0, cols), dtype=torch.bfloat16 if _has_combine_kernel(rows) else rows.dtype, device=rows.device)
     if pos is not None:
-        rows = _never_empty(rows)
+        rows, pos = _never_empty(rows), pos.reshape(-1)[: tokens * top_k]      # a table may be longer than the batch
     if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():
         y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
         w = weights.to(torch.float32).contiguous()

@@ -53,3 +53,12 @@ def test_cpu_combine_does_not_look_at_the_weight_of_a_missing_row():
     da, dw = torch.autograd.grad(y, (a, w), torch.ones(2, 3))
     assert da.tolist() == [[0.0] * 3, [0.5] * 3, [0.0] * 3, [2.0] * 3]
     assert dw.tolist() == [[float(rows[1].sum()), 0.0], [0.0, float(rows[3].sum())]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_cpu_combine_takes_a_table_longer_than_the_batch(dtype):
+    rows, w = torch.arange(12.0).view(4, 3).to(dtype), torch.tensor([[0.5, 1.0], [0.25, 2.0]])
+    short = torch.tensor([3, 0, -1, 2])
+    want = moe_ops.combine_topk(rows, short, w, 2, 2)
+    assert torch.equal(moe_ops.combine_topk(rows, torch.cat([short, torch.tensor([1, 1, -1])]), w, 2, 2), want)
+    assert torch.equal(moe_ops.combine_topk(rows, short.view(2, 2), w, 2, 2), want)
