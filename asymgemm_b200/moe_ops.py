@@ -172,6 +172,8 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
                                                    tokens, top_k, cols, _stream(rows)))
         return y
     if rows.is_cuda and rows.dtype == torch.float32 and cols % 4 == 0 and rows.is_contiguous():
+        if pos is None:
+            pos = torch.arange(tokens * top_k, device=rows.device)
         y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
         w = weights.to(torch.float32).contiguous()
         with torch.cuda.device(rows.device):

@@ -56,3 +56,14 @@ def test_the_combine_of_an_empty_batch_has_the_type_of_any_other(dtype, cols):
     for fn in (moe_ops.combine_topk, moe_ops.combine_topk_forward):
         full, empty = fn(rows, pos, w, 4, 2), fn(rows, pos[:0], w[:0], 0, 2)
         assert empty.shape == (0, cols) and empty.dtype == full.dtype
+
+
+@pytest.mark.parametrize("dtype,cols", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float32, 12), (torch.float16, 64)])
+def test_combine_without_a_position_table(dtype, cols):
+    rows, w = randn(14, cols, seed=5, dtype=dtype), torch.rand((4, 3), device=DEV)
+    y = moe_ops.combine_topk(rows, None, w, 4, 3)
+    assert torch.equal(y, moe_ops.combine_topk(rows, torch.arange(12, device=DEV), w, 4, 3))
+    want = (rows[:12].double().view(4, 3, cols) * w.double().unsqueeze(2)).sum(1)
+    size = (rows[:12].double().view(4, 3, cols) * w.double().unsqueeze(2)).abs().sum(1)
+    # three products and additions in fp32, one rounding
+    assert bool(((y.double() - want).abs() <= size * 6 * 2 ** -24 + want.abs() * torch.finfo(y.dtype).eps / 2).all())

@@ -52,7 +52,7 @@ def test_cpu_combine_does_not_look_at_the_weight_of_a_missing_row():
     assert torch.equal(y, torch.stack([0.5 * rows[1], 2 * rows[3]]))
     da, dw = torch.autograd.grad(y, (a, w), torch.ones(2, 3))
     assert da.tolist() == [[0.0] * 3, [0.5] * 3, [0.0] * 3, [2.0] * 3]
-    assert dw.tolist() == [[float(rows[1].sum()), 0.0], [0.0, float(rows[3].sum())]]
+    assert dw.tolist() == [[float(rows[1].detach().sum()), 0.0], [0.0, float(rows[3].detach().sum())]]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
