@@ -146,6 +146,16 @@ def _has_combine_kernel(rows: torch.Tensor) -> bool:
     return rows.is_cuda and rows.is_contiguous() and rows.shape[1] % {torch.bfloat16: 8, torch.float32: 4}.get(rows.dtype, 1 << 62) == 0
 
 
+def _check_combine_tables(rows, pos, weights, pairs: int) -> None:
+    """What the kernels read by address: wrong types or too few entries would be read past their end."""
+    if pos is not None and not (pos.dtype == torch.int64 and pos.device == rows.device and pos.is_contiguous() and pos.numel() >= pairs):
+        raise RuntimeError(f"pos must be a contiguous int64 tensor of {pairs} entries at least, on the device of rows")
+    if pos is None and rows.shape[0] < pairs:
+        raise RuntimeError(f"without pos, rows must hold a row for each of the {pairs} slots")
+    if weights.device != rows.device or weights.numel() < pairs:
+        raise RuntimeError(f"weights must hold {pairs} entries on the device of rows")
+
+
 def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (bf16 where a CUDA kernel runs); pos
     None = t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
@@ -164,6 +174,8 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
         return torch.empty((0, cols), dtype=torch.bfloat16 if _has_combine_kernel(rows) else rows.dtype, device=rows.device)
     if pos is not None:
         rows, pos = _never_empty(rows), pos.reshape(-1)[: tokens * top_k]      # a table may be longer than the batch
+    if _has_combine_kernel(rows):
+        _check_combine_tables(rows, pos, weights, tokens * top_k)
     if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():
         y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
         w = weights.to(torch.float32).contiguous()

@@ -67,3 +67,16 @@ def test_combine_without_a_position_table(dtype, cols):
     size = (rows[:12].double().view(4, 3, cols) * w.double().unsqueeze(2)).abs().sum(1)
     # three products and additions in fp32, one rounding
     assert bool(((y.double() - want).abs() <= size * 6 * 2 ** -24 + want.abs() * torch.finfo(y.dtype).eps / 2).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_combine_refuses_tables_that_its_kernels_would_read_past(dtype):
+    rows, pos, w = randn(16, 64, seed=6, dtype=dtype), torch.arange(12, device=DEV), torch.rand((6, 2), device=DEV)
+    want = moe_ops.combine_topk(rows, pos, w, 6, 2)
+    for bad in ((rows, pos.int(), w), (rows, pos[:11], w), (rows, pos.cpu(), w), (rows, torch.arange(24, device=DEV)[::2], w), (rows, pos, w[:5]), (rows, pos, w.cpu()),
+                (rows[:11], None, w)):
+        for grad in (False, True):
+            with pytest.raises(RuntimeError):
+                moe_ops.combine_topk(bad[0].clone().requires_grad_(grad), bad[1], bad[2], 6, 2)
+    assert torch.equal(moe_ops.combine_topk(rows, pos.view(6, 2), w, 6, 2), want)
+    assert torch.equal(moe_ops.combine_topk(rows, pos, torch.cat([w, w]), 6, 2), want)
