@@ -159,8 +159,8 @@ def _check_combine_tables(rows, pos, weights, pairs: int) -> None:
 def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, tokens: int, top_k: int) -> torch.Tensor:
     """y[t] = sum_j weights[t, j] * rows[pos[t*top_k + j]] (fp32 accumulation), as rows.dtype (bf16 where a CUDA kernel runs); pos
     None = t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
-    `weights`; where the CUDA kernels run (contiguous rows, bf16 with cols a multiple of 8 or fp32 with a multiple of 4) the
-    gradient is `combine_topk_backward`'s: no two slots may name the same row, and cols must be a multiple of 8."""
+    `weights`; where the CUDA kernels run (contiguous rows, bf16 or fp32, cols a multiple of 8) the gradient is
+    `combine_topk_backward`'s: no two slots may name the same row. Elsewhere it is plain torch's."""
     if _has_combine_kernel(rows) and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
     return combine_topk_forward(rows, pos, weights, tokens, top_k)
@@ -170,34 +170,31 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
     """`combine_topk` without a record for autograd where the CUDA kernels run: the layers' inference path, whose GEMMs have none
     either and whose buffers the next call overwrites."""
     cols = rows.shape[1]
+    if not _has_combine_kernel(rows):
+        return _combine_plain(rows, pos, weights, tokens, top_k).to(rows.dtype)
     if tokens == 0:
-        return torch.empty((0, cols), dtype=torch.bfloat16 if _has_combine_kernel(rows) else rows.dtype, device=rows.device)
+        return torch.empty((0, cols), dtype=torch.bfloat16, device=rows.device)
     if pos is not None:
         rows, pos = _never_empty(rows), pos.reshape(-1)[: tokens * top_k]      # a table may be longer than the batch
-    if _has_combine_kernel(rows):
-        _check_combine_tables(rows, pos, weights, tokens * top_k)
-    if rows.is_cuda and rows.dtype == torch.bfloat16 and cols % 8 == 0 and rows.is_contiguous():
-        y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
-        w = weights.to(torch.float32).contiguous()
-        with torch.cuda.device(rows.device):
-            _lib.check(_lib.load().ag_combine_topk(rows.data_ptr(), pos.data_ptr() if pos is not None else None, w.data_ptr(), y.data_ptr(),
-                                                   tokens, top_k, cols, _stream(rows)))
-        return y
-    if rows.is_cuda and rows.dtype == torch.float32 and cols % 4 == 0 and rows.is_contiguous():
-        if pos is None:
-            pos = torch.arange(tokens * top_k, device=rows.device)
-        y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
-        w = weights.to(torch.float32).contiguous()
-        with torch.cuda.device(rows.device):
-            _lib.check(_lib.load().ag_combine_topk_f32(rows.data_ptr(), pos.data_ptr(), w.data_ptr(), y.data_ptr(), tokens, top_k, cols,
-                                                       _stream(rows)))
-        return y
-    picked = (rows.index_select(0, pos.clamp(min=0)) if pos is not None else rows[: tokens * top_k]).view(tokens, top_k, cols).float()
-    w = weights.reshape(tokens, top_k, 1).float()
-    if pos is not None:      # what has no row adds nothing, whatever its weight and row 0 are
-        none = (pos < 0).view(tokens, top_k, 1)
-        picked, w = picked.masked_fill(none, 0), w.masked_fill(none, 0)
-    return (picked * w).sum(dim=1).to(rows.dtype)
+    _check_combine_tables(rows, pos, weights, tokens * top_k)
+    if rows.dtype == torch.float32 and pos is None:
+        pos = torch.arange(tokens * top_k, device=rows.device)
+    y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
+    w = weights.to(torch.float32).contiguous()
+    with torch.cuda.device(rows.device):
+        combine = _lib.load().ag_combine_topk if rows.dtype == torch.bfloat16 else _lib.load().ag_combine_topk_f32
+        _lib.check(combine(rows.data_ptr(), pos.data_ptr() if pos is not None else None, w.data_ptr(), y.data_ptr(), tokens, top_k, cols, _stream(rows)))
+    return y
+
+
+def _combine_plain(rows, pos, weights, tokens: int, top_k: int) -> torch.Tensor:
+    """The sum in plain torch, fp32: types and widths without a kernel, and CPU tensors."""
+    if pos is None:
+        return (rows[: tokens * top_k].reshape(tokens, top_k, rows.shape[1]).float() * weights.reshape(tokens, top_k, 1).float()).sum(dim=1)
+    pos = pos.reshape(-1)[: tokens * top_k]      # a table may be longer than the batch
+    none = (pos < 0).view(tokens, top_k, 1)      # what has no row adds nothing, whatever its weight and row 0 are
+    picked = _never_empty(rows).index_select(0, pos.clamp(min=0)).view(tokens, top_k, rows.shape[1])
+    return (picked.float().masked_fill(none, 0) * weights.reshape(tokens, top_k, 1).float().masked_fill(none, 0)).sum(dim=1)
 
 
 def combine_topk_backward(dy: torch.Tensor, rows: torch.Tensor, pos: Optional[torch.Tensor], weights: torch.Tensor, need_rows: bool = True,
@@ -223,6 +220,12 @@ class _CombineTopK(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         rows, pos, weights = ctx.saved_tensors
+        if rows.shape[1] % 8:      # fp32 rows of 4 mod 8 columns: the forward pass has a kernel, the gradient has none
+            with torch.enable_grad():
+                leaves = [rows.detach().requires_grad_(True), weights.detach().requires_grad_(True)]
+                y = _combine_plain(leaves[0], pos, leaves[1], dy.shape[0], ctx.top_k)
+            grads = torch.autograd.grad(y, [t for t, need in zip(leaves, (ctx.needs_input_grad[0], ctx.needs_input_grad[2])) if need], dy.float())
+            return grads[0] if ctx.needs_input_grad[0] else None, None, grads[-1] if ctx.needs_input_grad[2] else None, None, None
         if pos is not None:
             pos = pos[: weights.numel()]      # a table may be longer than the batch
         drows, dweights = combine_topk_backward(dy.contiguous(), rows, pos, weights.reshape(dy.shape[0], ctx.top_k), ctx.needs_input_grad[0],

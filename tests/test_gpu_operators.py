@@ -80,3 +80,33 @@ def test_combine_refuses_tables_that_its_kernels_would_read_past(dtype):
                 moe_ops.combine_topk(bad[0].clone().requires_grad_(grad), bad[1], bad[2], 6, 2)
     assert torch.equal(moe_ops.combine_topk(rows, pos.view(6, 2), w, 6, 2), want)
     assert torch.equal(moe_ops.combine_topk(rows, pos, torch.cat([w, w]), 6, 2), want)
+
+
+@pytest.mark.parametrize("cols", [4, 12, 20, 1028])
+@pytest.mark.parametrize("table", [True, False])
+def test_gradient_of_the_combine_at_widths_where_only_the_sum_has_a_kernel(cols, table):
+    """fp32 rows of 4 mod 8 columns."""
+    tokens, k = 7, 3
+    rows, w = randn(40, cols, seed=7), torch.rand((tokens, k), generator=torch.Generator().manual_seed(8)).to(DEV)
+    pos = torch.randperm(40, generator=torch.Generator().manual_seed(9))[: tokens * k].to(DEV) if table else None
+    if table:
+        pos[::5] = -1
+    dy = randn(tokens, cols, seed=10, dtype=torch.bfloat16)
+    a, b = rows.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = moe_ops.combine_topk(a, pos, b, tokens, k)
+    assert torch.equal(y.detach(), moe_ops.combine_topk(rows, pos, w, tokens, k))
+    drows, dweights = torch.autograd.grad(y, (a, b), dy, retain_graph=True)
+    at = pos if table else torch.arange(tokens * k, device=DEV)
+    live = at >= 0
+    g = dy.double().repeat_interleave(k, 0)
+    want = torch.zeros(rows.shape, dtype=torch.float64, device=DEV)
+    want[at[live]] = (w.double().view(-1, 1) * g)[live]
+    assert drows.dtype == torch.float32 and bool(((drows.double() - want).abs() <= want.abs() * 2 ** -23).all())
+    terms = torch.where(live.unsqueeze(1), rows.double()[at.clamp(min=0)] * g, 0)
+    # a product and at most `cols` additions in fp32
+    assert bool(((dweights.double().view(-1) - terms.sum(1)).abs() <= terms.abs().sum(1) * (cols + 1) * 2 ** -24).all())
+    assert torch.equal(torch.autograd.grad(y, a, dy, retain_graph=True)[0], drows) and torch.equal(torch.autograd.grad(y, b, dy)[0], dweights)
+    assert torch.equal(torch.autograd.grad(moe_ops.combine_topk(rows, pos, b, tokens, k), b, dy)[0], dweights)
+    assert torch.equal(torch.autograd.grad(moe_ops.combine_topk(a, pos, w, tokens, k), a, dy)[0], drows)
+    empty = moe_ops.combine_topk(a, None if pos is None else pos[:0], b[:0], 0, k)
+    assert empty.shape == (0, cols) and float(torch.autograd.grad(empty.sum(), a)[0].abs().max()) == 0
