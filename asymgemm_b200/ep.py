@@ -28,6 +28,7 @@ import torch.distributed as dist
 from . import moe_ops
 
 ALIGN = 128
+MAX_HISTOGRAM_EXPERTS = 8192      # experts that ag_ep_histogram counts
 
 
 @dataclass
@@ -88,11 +89,24 @@ class EPDispatcher:
         """Sort the (token, slot) pairs by expert and exchange per-expert counts.
 
         Returns (order [T*k], send_counts int32 [world, max_experts_per_rank], recv_counts int32 [world, experts_per_rank]),
-        recv_counts[s, j] = rows rank s sends to this rank's local expert j.
+        recv_counts[s, j] = rows rank s sends to this rank's local expert j. Pairs without an expert (id -1) come last in the order
+        and count nowhere. So do ids outside the experts on a GPU, where they set the status word (`check_status` raises); where the
+        host sees the ids they raise here.
         """
-        flat = topk_ids.reshape(-1)
-        order = torch.argsort(flat, stable=True)
-        per_expert = torch.bincount(flat, minlength=self.num_experts)
+        flat = topk_ids.reshape(-1).to(torch.int64).contiguous()
+        known = (flat >= 0) & (flat < self.num_experts)
+        key = torch.where(known, flat, self.num_experts)
+        order = torch.argsort(key, stable=True)
+        if flat.is_cuda and flat.numel() and self.num_experts <= MAX_HISTOGRAM_EXPERTS:
+            from . import _lib, api
+            per_expert = torch.empty(self.num_experts, dtype=torch.int32, device=flat.device)
+            with torch.cuda.device(flat.device):
+                _lib.check(_lib.load().ag_ep_histogram(flat.data_ptr(), flat.numel(), self.num_experts, per_expert.data_ptr(),
+                                                       api._status_word(flat.device).data_ptr(), torch.cuda.current_stream(flat.device).cuda_stream))
+        else:
+            if bool((~known & (flat != -1)).any()):
+                raise RuntimeError(f"the routing names an expert id outside [0, {self.num_experts})")
+            per_expert = torch.bincount(key, minlength=self.num_experts + 1)[: self.num_experts]
         slot = self._slot_cache.get(flat.device)
         if slot is None:
             slot = self._slot_expert.to(flat.device)
@@ -103,7 +117,7 @@ class EPDispatcher:
         self._all_to_all(recv_counts, send_counts)
         return order, send_counts, recv_counts[:, : self.experts_per_rank].contiguous()
 
-    def layout(self, recv_counts: torch.Tensor, total_recv: int):
+    def layout(self, recv_counts: torch.Tensor, total_recv: int, missing: bool = False):
         """Contiguous layout of the received rows: grouped by local expert, each expert padded to 128 rows.
 
         Pure tensor arithmetic on the device of `recv_counts` [world, experts_per_rank] -- no host synchronisation.
@@ -111,6 +125,7 @@ class EPDispatcher:
         padded_bound, offsets int32 [2*epr], experts int32 [epr+1]): dest_rows[i] = row of received row i in the padded
         layout; every local expert gets a segment (an empty one if it received nothing, which the GEMM skips);
         padded_bound = total_recv rounded up plus 127 rows per expert, an upper bound of the rows the layout can use.
+        `missing`: total_recv may be more than the rows counted; the rest, at the end, has no row (dest_rows -1).
         """
         dev = recv_counts.device
         epr = int(recv_counts.shape[1])       # all local experts, or one group of them (pipelined)
@@ -122,8 +137,13 @@ class EPDispatcher:
         block_dest = (expert_start.unsqueeze(0) + within).reshape(-1)    # [world*epr], source-major like the recv order
         block_len = rc.reshape(-1)
         block_recv = torch.cumsum(block_len, 0) - block_len
-        shift = torch.repeat_interleave(block_dest - block_recv, block_len, output_size=total_recv)
-        dest_rows = shift + torch.arange(total_recv, device=dev)
+        block_shift, received = block_dest - block_recv, torch.arange(total_recv, device=dev)
+        if missing:      # one more block takes what is left
+            counted = block_len.sum().view(1)
+            block_len, block_shift = torch.cat([block_len, total_recv - counted]), torch.cat([block_shift, block_shift.new_zeros(1)])
+        dest_rows = torch.repeat_interleave(block_shift, block_len, output_size=total_recv) + received
+        if missing:
+            dest_rows = torch.where(received < counted, dest_rows, -1)
         offsets = torch.stack([expert_start, expert_start + padded], dim=1).reshape(-1).to(torch.int32)
         experts = torch.cat([torch.arange(epr, device=dev, dtype=torch.int32), torch.full((1,), -1, device=dev, dtype=torch.int32)])
         padded_bound = (total_recv + ALIGN - 1) // ALIGN * ALIGN + epr * ALIGN if total_recv > 0 else 0
@@ -136,7 +156,11 @@ class EPDispatcher:
         Returns (state, recv_rows [R, H], recv_extras). With one rank nothing leaves the device and the host never
         waits; with several ranks the split sizes of the exchange are read back once, on a side stream, so the host
         does not wait for GEMMs still running on the compute stream. On one GPU the layout comes from `moe_ops.route_layout`
-        (one or two kernels; pairs with id -1, as `moe_ops.route_topk` marks padding tokens, get no row).
+        (one or two kernels).
+
+        Pairs with id -1, as `moe_ops.route_topk` marks padding tokens, get no row and are sent nowhere. Other ids outside the
+        experts raise on CPU tensors; on a GPU, where no host waits for the ids, their pairs are left out in the same way and the
+        status word is set: `check_status` raises, and nothing here calls it.
         """
         tokens, top_k = topk_ids.shape
         if self.world == 1 and topk_ids.is_cuda and self.num_experts <= moe_ops.MAX_LAYOUT_EXPERTS and topk_ids.dtype in (torch.int64, torch.int32):
@@ -162,6 +186,7 @@ class EPDispatcher:
                 counts_host = torch.stack([send_counts.sum(dim=1), recv_counts.sum(dim=1)]).cpu()
             send_splits, recv_splits = counts_host[0].tolist(), counts_host[1].tolist()
             total_recv = int(sum(recv_splits))
+            order = order[: sum(send_splits)]      # the pairs that have an expert
         src_token = torch.div(order, top_k, rounding_mode="floor")
         outs = []
         for t in (rows,) + tuple(extras):
@@ -173,7 +198,7 @@ class EPDispatcher:
             recv = torch.empty((total_recv,) + tuple(as_bytes.shape[1:]), dtype=as_bytes.dtype, device=as_bytes.device)
             self._all_to_all(recv, as_bytes, recv_splits, send_splits)
             outs.append(recv.view(t.dtype) if t.dtype == torch.float8_e4m3fn else recv)
-        dest_rows, per_expert, padded_rows, offsets, experts = self.layout(recv_counts, total_recv)
+        dest_rows, per_expert, padded_rows, offsets, experts = self.layout(recv_counts, total_recv, missing=self.world == 1)
         state = DispatchState(order, send_splits, recv_splits, dest_rows, per_expert, padded_rows, offsets, experts, tokens, top_k,
                               src_token if self.world == 1 else None)
         return state, outs[0], tuple(outs[1:])
@@ -205,6 +230,7 @@ class EPDispatcher:
         with on_comm():
             order, send_counts, recv_counts = self.plan(topk_ids)
             send_host, recv_host = send_counts.cpu().to(torch.int64), recv_counts.cpu().to(torch.int64)   # waits for this stream only
+            order = order[: int(send_host.sum())]      # the pairs that have an expert
             src_token = torch.div(order, top_k, rounding_mode="floor")
         groups = max(1, min(int(groups), min(hi - lo for lo, hi in self.expert_ranges)))
         # the (token, slot) pairs sorted by expert are also sorted by (rank, local expert): start of every such block
@@ -273,11 +299,17 @@ class EPDispatcher:
             keep += [out, back, ret, state]          # alive until both streams are done with them
         if cuda:
             main.wait_stream(comm)
-        inv = torch.empty_like(order)
-        inv[order] = torch.arange(order.numel(), device=dev)
+        inv = self._inverse(order, tokens * top_k)
         y = moe_ops.combine_topk_forward(ret_sorted, inv, topk_weights, tokens, top_k)
         del keep
         return y
+
+    @staticmethod
+    def _inverse(order: torch.Tensor, pairs: int) -> torch.Tensor:
+        """Inverse of the sort: pair p (token p // k, slot p % k) was sent as sorted row inv[p]; -1 for pairs that were not."""
+        inv = torch.empty_like(order) if order.numel() == pairs else order.new_full((pairs,), -1)
+        inv[order] = torch.arange(order.numel(), device=order.device)
+        return inv
 
     def _side_stream(self, device):
         if device.type != "cuda":
@@ -293,9 +325,7 @@ class EPDispatcher:
             if mark is not None:
                 mark("return")
             return moe_ops.combine_topk_forward(expert_out, state.tables.pair_row, topk_weights, state.tokens, state.top_k)
-        # inverse of the sort: pair p (token p // k, slot p % k) was sent as sorted row inv[p]
-        inv = torch.empty_like(state.order)
-        inv[state.order] = torch.arange(state.order.numel(), device=state.order.device)
+        inv = self._inverse(state.order, state.tokens * state.top_k)
         if self.world == 1:
             # the sorted rows never left this rank: read them straight out of the padded layout
             pos = state.dest_rows.index_select(0, inv)
@@ -303,7 +333,7 @@ class EPDispatcher:
                 mark("return")
             return moe_ops.combine_topk_forward(expert_out, pos, topk_weights, state.tokens, state.top_k)
         back = moe_ops.move_rows(expert_out, state.dest_rows.numel(), src_rows=state.dest_rows)
-        ret = torch.empty((state.tokens * state.top_k, back.shape[1]), dtype=back.dtype, device=back.device)
+        ret = torch.empty((state.order.numel(), back.shape[1]), dtype=back.dtype, device=back.device)
         self._all_to_all(ret, back, state.send_splits, state.recv_splits)
         if mark is not None:
             mark("return")

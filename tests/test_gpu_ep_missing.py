@@ -150,3 +150,41 @@ def test_pairs_without_room_are_left_out_of_the_combine():
     assert torch.equal(a.body.view(cap, 64)[pair_row[kept]], x[kept])
     for g in (a, s, meta, ret):
         g.check()
+
+
+@pytest.mark.parametrize("experts,dtype", [(1100, torch.int64), (6, torch.int16), (6, torch.int64)])
+def test_dispatcher_on_one_gpu_without_and_with_the_layout_kernels(experts, dtype):
+    """More experts than the layout kernels take, and ids of a type that they do not: laid out by torch, without a host wait."""
+    tokens, k, cols = 50, 3, 64
+    gen = torch.Generator().manual_seed(70)
+    ids = torch.randint(0, experts, (tokens, k), generator=gen)
+    ids[torch.rand(ids.shape, generator=gen) < 0.3] = -1
+    ids[40:] = -1
+    x = torch.randn((tokens, cols), generator=gen).to(torch.bfloat16)
+    w = torch.rand((tokens, k), generator=gen)
+    w[ids < 0] = float("nan")
+    disp = ep.EPDispatcher(experts)
+    state, recv, _ = disp.dispatch(x.to(DEV), ids.to(dtype).to(DEV))
+    want_state, want_recv, _ = ep.EPDispatcher(experts).dispatch(x, ids)
+    assert (state.tables is None) == (experts > 1024 or dtype == torch.int16)
+    a, want_a = ep.to_contiguous_layout(recv, state), ep.to_contiguous_layout(want_recv, want_state)
+    assert torch.equal(a.cpu(), want_a) and torch.equal(state.offsets.cpu(), want_state.offsets)
+    y = disp.combine(a, state, w.to(DEV)).cpu()
+    want = torch.where(ids < 0, 0, w).double().sum(1, keepdim=True) * x.double()
+    # k products and additions in fp32, one rounding to bf16
+    assert bool(((y.double() - want).abs() <= want.abs() * (2 ** -8 + 2 * k * 2 ** -24)).all())
+
+
+@pytest.mark.expects_status
+@pytest.mark.parametrize("experts", [6, 1100])
+def test_ids_outside_the_experts_are_dropped_and_reported_by_the_dispatcher(experts):
+    ids = torch.tensor([[0, experts], [-2, 1], [3, -1]], device=DEV)
+    x = torch.ones((3, 64), dtype=torch.bfloat16, device=DEV)
+    disp = ep.EPDispatcher(experts)
+    state, recv, _ = disp.dispatch(x, ids)
+    assert int(state.rows_per_expert.sum()) == 3
+    y = disp.combine(ep.to_contiguous_layout(recv, state), state, torch.ones((3, 2), device=DEV))
+    assert y[:, 0].tolist() == [1.0, 1.0, 1.0]
+    with pytest.raises(RuntimeError, match="expert id"):
+        ag.check_status()
+    ag.check_status()

@@ -6,6 +6,8 @@ import pytest
 import torch
 
 from asymgemm_b200 import ep_peer, moe_ops
+from asymgemm_b200.ep import EPDispatcher, to_contiguous_layout
+from tests import test_ep_gloo as gloo
 
 
 @pytest.mark.parametrize("world", [1, 2])
@@ -62,3 +64,71 @@ def test_cpu_combine_takes_a_table_longer_than_the_batch(dtype):
     want = moe_ops.combine_topk(rows, short, w, 2, 2)
     assert torch.equal(moe_ops.combine_topk(rows, torch.cat([short, torch.tensor([1, 1, -1])]), w, 2, 2), want)
     assert torch.equal(moe_ops.combine_topk(rows, short.view(2, 2), w, 2, 2), want)
+
+
+# ------------------------------------------------------------------------------------------------------ exchange between ranks
+def _missing_ids(rank, tokens, experts, k):
+    """What the router gives: -1 where a row has too few live experts and in the padding tokens at the end; rank 2 has nothing else."""
+    gen = torch.Generator().manual_seed(200 + rank)
+    ids = torch.stack([torch.randperm(experts, generator=gen)[:k] for _ in range(tokens)])
+    ids[torch.rand(ids.shape, generator=gen) < 0.2] = -1
+    ids[tokens - 5:] = -1
+    return torch.full_like(ids, -1) if rank == 2 else ids
+
+
+def _missing_worker(rank, world, port, q):
+    try:
+        gloo._init(rank, world, port)
+        experts, tokens, hidden, k = 12, 31 + 4 * rank, 16, 3
+        x = torch.randn((tokens, hidden), generator=torch.Generator().manual_seed(rank))
+        x[tokens - 5:] = float("nan")
+        ids = _missing_ids(rank, tokens, experts, k)
+        w = torch.rand((tokens, k), generator=torch.Generator().manual_seed(50 + rank))
+        w[ids < 0] = float("nan")
+        want = torch.where(ids < 0, 0, (ids + 1).float() * w).sum(dim=1, keepdim=True) * torch.nan_to_num(x)
+        tag = torch.arange(tokens, dtype=torch.float32).unsqueeze(1)
+        disp = EPDispatcher(experts)
+        first = disp.expert_ranges[rank][0]
+        state, recv, (recv_tag,) = disp.dispatch(x, ids, (tag,))
+        assert sum(state.send_splits) == int((ids >= 0).sum()) and recv.shape[0] == recv_tag.shape[0] == int(state.rows_per_expert.sum()) == sum(state.recv_splits)
+        y = disp.combine(gloo._fake_experts(to_contiguous_layout(recv, state), state, first), state, w)
+        assert torch.allclose(y, want, rtol=1e-5, atol=1e-5), (y - want).abs().max()
+        for groups in (1, 2, 3):
+            def group_fn(rows, extras, st, start, count):
+                return gloo._fake_experts(to_contiguous_layout(rows, st), st, first + start)
+
+            y = disp.pipelined(x, (tag,), ids, w, groups, group_fn)
+            assert torch.allclose(y, want, rtol=1e-5, atol=1e-5), (groups, (y - want).abs().max())
+        torch.distributed.barrier()
+        q.put((rank, "ok"))
+    except Exception as e:  # pragma: no cover - reported through the queue
+        q.put((rank, f"error: {type(e).__name__}: {e}"))
+    finally:
+        if torch.distributed.is_initialized():
+            torch.distributed.destroy_process_group()
+
+
+@pytest.mark.parametrize("world", [2, 3])
+def test_ranks_exchange_no_row_for_pairs_without_an_expert(world):
+    results = gloo._run(_missing_worker, world=world)
+    assert results == {r: "ok" for r in range(world)}, results
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16])
+def test_one_rank_gives_pairs_without_an_expert_no_row(dtype):
+    disp = EPDispatcher(4)
+    ids = torch.tensor([[0, 3], [-1, 1], [3, -1], [-1, -1]], dtype=dtype)
+    x = torch.arange(4, dtype=torch.float32).unsqueeze(1) + 1
+    state, recv, _ = disp.dispatch(x, ids)
+    assert state.rows_per_expert.tolist() == [1, 1, 0, 2]
+    a = to_contiguous_layout(recv, state)
+    assert a[0, 0] == 1 and a[128, 0] == 2 and a[256:258, 0].tolist() == [1.0, 3.0] and float(a.abs().sum()) == 7
+    w = torch.tensor([[1.0, 1.0], [float("nan"), 1.0], [1.0, float("inf")], [float("nan")] * 2])
+    assert disp.combine(a, state, w).view(-1).tolist() == [2.0, 2.0, 3.0, 0.0]
+    state, recv, _ = disp.dispatch(x, torch.full_like(ids, -1))
+    a = to_contiguous_layout(recv, state)
+    assert float(a.abs().sum()) == 0 and float(disp.combine(a, state, w).abs().sum()) == 0
+    for bad in (4, -2, 100):
+        ids[1, 1] = bad
+        with pytest.raises(RuntimeError, match="expert id"):
+            disp.dispatch(x, ids)
