@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
@@ -1155,6 +1156,18 @@ long long layout_run(long long pairs) {
   return (least + agb::kLayoutThreads - 1) / agb::kLayoutThreads * agb::kLayoutThreads;
 }
 
+// Shared memory of the placing kernel. Its limit is raised once per device, for the most experts: the limit belongs to the function,
+// so a call that set it to its own needs could lower it between another thread's setting and launch.
+constexpr size_t layout_memory(int experts) { return (static_cast<size_t>(experts) * (3 + agb::kLayoutWarps) + 1) * 4; }
+cudaError_t allow_layout_memory(void (*place)(agb::LayoutParams), std::atomic<bool> (&allowed)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && allowed[dev].load(std::memory_order_relaxed))) return e;
+  e = cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(layout_memory(agb::kLayoutMaxExperts)));
+  if (e == cudaSuccess && dev < 64) allowed[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1289,17 +1302,15 @@ int ag_route_layout(const ag_route_layout_desc_t* r) {
   p.status = r->status;
   p.run = run;
   cudaStream_t stream = static_cast<cudaStream_t>(r->stream);
-  const size_t smem = (static_cast<size_t>(r->experts) * (3 + agb::kLayoutWarps) + 1) * 4;
   auto place = blocks == 1 ? agb::layout_place_kernel<true> : agb::layout_place_kernel<false>;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
-  }
+  static std::atomic<bool> allowed[2][64];
+  const cudaError_t e = allow_layout_memory(place, allowed[blocks == 1]);
+  if (e != cudaSuccess) return agb_fail(AG_E_CUDA, cudaGetErrorString(e));
   if (blocks > 1) agb::layout_count_kernel<<<blocks, agb::kLayoutThreads, static_cast<size_t>(r->experts) * 4, stream>>>(p);
   // few pairs: a block more for every kLayoutFill rows to be marked (64 pairs x 8, 256 experts, 33280 rows: 10.5 us on one block, 6.6 on 9)
   const int64_t fill = (r->rows + kLayoutFill - 1) / kLayoutFill;
   const int grid = blocks > 1 ? blocks : fill < 1 ? 1 : fill > 64 ? 64 : static_cast<int>(fill);
-  place<<<grid, agb::kLayoutThreads, smem, stream>>>(p);
+  place<<<grid, agb::kLayoutThreads, layout_memory(r->experts), stream>>>(p);
   return launch_check();
 }
 

@@ -1,6 +1,7 @@
 """Operators around the grouped GEMMs where calls are unusual: nothing to do, tables longer than the batch, widths and types without
 a kernel, calls recorded into graphs, derivatives that are not there."""
-import math
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -110,3 +111,44 @@ def test_gradient_of_the_combine_at_widths_where_only_the_sum_has_a_kernel(cols,
     assert torch.equal(torch.autograd.grad(moe_ops.combine_topk(a, pos, w, tokens, k), a, dy)[0], drows)
     empty = moe_ops.combine_topk(a, None if pos is None else pos[:0], b[:0], 0, k)
     assert empty.shape == (0, cols) and float(torch.autograd.grad(empty.sum(), a)[0].abs().max()) == 0
+
+
+LAYOUTS_AT_THE_SHARED_MEMORY_LIMIT = """
+import threading, torch
+import asymgemm_b200 as ag
+from asymgemm_b200 import moe_ops
+
+def check(tokens, experts):
+    ids = torch.randint(-1, experts, (tokens, 2), generator=torch.Generator().manual_seed(experts))
+    got = moe_ops.route_layout(ids.cuda(), experts, 1)
+    flat = ids.view(-1)
+    order = torch.argsort(torch.where(flat < 0, experts, flat), stable=True)[: int((flat >= 0).sum())]
+    want = torch.full((flat.numel(),), -1)
+    want[order] = torch.arange(order.numel())
+    assert torch.equal(got.pair_row.cpu(), want), (tokens, experts)
+    assert torch.equal(got.rows_per_expert.cpu(), torch.bincount(flat[flat >= 0], minlength=experts)), (tokens, experts)
+
+for tokens in (700, 2500):          # one block, several
+    for experts in (351, 350, 352, 1024, 351):
+        check(tokens, experts)
+failed = []
+def many(experts):
+    try:
+        for _ in range(60):
+            check(700, experts)
+            check(2500, experts)
+    except Exception as e:
+        failed.append((experts, repr(e)))
+threads = [threading.Thread(target=many, args=(e,)) for e in (360, 1024, 500, 20)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert not failed, failed
+ag.check_status()
+print("done")
+"""
+
+
+def test_layouts_at_the_limit_of_shared_memory_and_from_several_threads():
+    """In a process of its own: 351 experts, whose tables just pass the default limit together with the kernel's own, come first."""
+    res = subprocess.run([sys.executable, "-c", LAYOUTS_AT_THE_SHARED_MEMORY_LIMIT], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.strip() == "done", res.stdout + res.stderr
