@@ -42,11 +42,6 @@ struct DenseParams {
   unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ float load_as_float(const void* p, long long i, int type) {
-  if (type == T_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  if (type == T_FP16) return __half2float(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
 __device__ __forceinline__ void store_from_float(void* p, long long i, int type, float v) {
   if (type == T_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else if (type == T_FP16) static_cast<__half*>(p)[i] = __float2half_rn(v);
