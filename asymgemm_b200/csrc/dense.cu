@@ -2,6 +2,8 @@
 // its gradients. Operands bf16 or fp16, fp32 accumulation, output in the operands' type or fp32; see dense_kernel.cuh.
 #include "dense_kernel.cuh"
 
+#include <atomic>
+
 #include "../../include/asymgemm_b200.h"
 
 int agb_fail(int code, const char* message);
@@ -238,20 +240,20 @@ Plan plan_product(const Operand& a, const Operand& b, int64_t steps, int sms) {
 }
 
 template <typename K>
-cudaError_t allow_shared_memory(K kernel, int bytes, bool (&configured)[64]) {
+cudaError_t allow_shared_memory(K kernel, int bytes, std::atomic<bool> (&configured)[64]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 0 && dev < 64 && configured[dev]) return cudaSuccess;
+  if (dev >= 0 && dev < 64 && configured[dev].load(std::memory_order_relaxed)) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev] = true;
+  if (e == cudaSuccess && dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_relaxed);
   return e;
 }
 
 template <bool A_MN, bool B_MN, bool ONE_CHUNK>
 cudaError_t launch_pair_as(const CUtensorMap& ma, const CUtensorMap& mb, const agb::DenseParams& p, int splits, int vector_width, int sms, cudaStream_t stream) {
   auto kernel = agb::dense_pair_kernel<A_MN, B_MN, ONE_CHUNK>;
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64];
   if (cudaError_t e = allow_shared_memory(kernel, agb::PairDenseSmem::dyn_bytes, configured)) return e;
   const int64_t items = (static_cast<int64_t>(p.rows_a) + agb::kPairTile - 1) / agb::kPairTile * p.tiles_b * splits;
   const int64_t pairs = sms / 2 < items ? sms / 2 : items;
@@ -264,7 +266,7 @@ cudaError_t launch_tile(const CUtensorMap& ma, const CUtensorMap& mb, const agb:
   using L = agb::TileSmem<BN>;
   static_assert(L::dyn_bytes * (BN >= 128 ? 1 : 2) <= 232448, "tile configuration does not fit in shared memory");
   auto kernel = agb::dense_tile_kernel<BN, A_MN, B_MN>;
-  static bool configured[64] = {};
+  static std::atomic<bool> configured[64];
   if (cudaError_t e = allow_shared_memory(kernel, L::dyn_bytes, configured)) return e;
   const int64_t tiles = (static_cast<int64_t>(p.rows_a) + agb::kTileA - 1) / agb::kTileA * p.tiles_b;
   cudaLaunchAttribute attr[1];
