@@ -164,6 +164,8 @@ def set_use_scratch(flag: bool) -> None:
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
+    if device.type != "cuda":      # it would be kept as the current GPU's
+        raise RuntimeError("asymgemm_b200: CUDA tensors are wanted")
     key = device.index if device.index is not None else torch.cuda.current_device()
     t = _status_cache.get(key)
     if t is None:

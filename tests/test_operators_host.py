@@ -5,7 +5,7 @@ import types
 import pytest
 import torch
 
-from asymgemm_b200 import ep_peer, moe_ops
+from asymgemm_b200 import api, dense_ops, ep_peer, moe_ops
 from asymgemm_b200.ep import EPDispatcher, to_contiguous_layout
 from tests import test_ep_gloo as gloo
 
@@ -132,3 +132,15 @@ def test_one_rank_gives_pairs_without_an_expert_no_row(dtype):
         ids[1, 1] = bad
         with pytest.raises(RuntimeError, match="expert id"):
             disp.dispatch(x, ids)
+
+
+def test_a_refused_cpu_tensor_leaves_no_status_word_behind(monkeypatch):
+    """The words are kept by GPU index, which a CPU tensor does not have: it must not become the current GPU's."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(api, "_status_cache", {})
+    x, ids = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((4, 2), dtype=torch.int64)
+    for call in (lambda: dense_ops.linear(x, x), lambda: dense_ops.linear_backward(x, x, x), lambda: moe_ops.route_layout(ids, 8),
+                 lambda: moe_ops.route_layout_masked(ids, 8, 4), lambda: moe_ops.combine_topk_backward(x, x, None, torch.zeros(4, 1))):
+        with pytest.raises(RuntimeError):
+            call()
+        assert not api._status_cache
