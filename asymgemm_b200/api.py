@@ -21,6 +21,7 @@ import weakref
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -172,6 +173,16 @@ def _status_word(device: torch.device) -> torch.Tensor:
         t = torch.zeros(1, dtype=torch.int32, device=device)
         _status_cache[key] = t
     return t
+
+
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation is under way and one of the tensors takes part (no level is open: -1, the usual case)."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    if _has_tangent(*tensors):
+        raise RuntimeError("asymgemm_b200: forward-mode derivatives are not supported here")
 
 
 def check_status(device: Union[torch.device, int, None] = None, reset: bool = True) -> None:

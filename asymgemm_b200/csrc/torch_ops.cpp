@@ -153,6 +153,13 @@ class Pieces {
 
 void check_ok(int rc) { TORCH_CHECK(rc == AG_OK, "asymgemm_b200: ", ag_last_error(), " (code ", rc, ")"); }
 
+// These operators have no forward-mode derivative (and are not recorded by autograd here): a tangent would be lost without a word.
+void no_tangents(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(t == nullptr || !t->defined() || !t->_fw_grad(0).defined(), "asymgemm_b200: forward-mode derivatives are not supported here");
+}
+const at::Tensor* get(const OptTensor& t) { return t.has_value() ? &*t : nullptr; }
+
 int32_t type_code(at::ScalarType t, const char* name) {
   if (t == at::kBFloat16) return AG_T_BF16;
   if (t == at::kHalf) return AG_T_FP16;
@@ -177,6 +184,7 @@ void check_same_device(const OptTensor& t, const char* name, const at::Tensor& a
 
 std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits, int64_t top_k, int64_t scoring, const OptTensor& bias, int64_t groups,
                                               int64_t top_groups, bool group_max, bool renormalize, double scale, const OptTensor& rows_used) {
+  no_tangents({&logits, get(bias)});
   check_rows(logits, "logits");
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   TORCH_CHECK(experts > 0 && experts <= 1024 && top_k > 0 && top_k <= 32, "route_topk wants 1 .. 1024 experts and top_k 1 .. 32");
@@ -211,6 +219,7 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits, int64_t 
 
 at::Tensor route_topk_backward(const at::Tensor& dweights, const at::Tensor& ids, const at::Tensor& logits, int64_t scoring, bool renormalize,
                                double scale) {
+  no_tangents({&dweights, &logits});
   check_rows(logits, "logits");
   TORCH_CHECK(ids.dim() == 2 && ids.size(0) == logits.size(0) && ids.size(1) > 0 && ids.size(1) <= 32, "topk_ids must be [tokens, top_k], top_k 1 .. 32");
   TORCH_CHECK(dweights.sizes() == ids.sizes(), "dweights must have the shape of topk_ids");
@@ -293,6 +302,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> route_layout_masked(const at::Ten
 
 std::tuple<at::Tensor, at::Tensor> combine_topk_backward(const at::Tensor& dy, const at::Tensor& rows, const OptTensor& pos, const at::Tensor& weights,
                                                          bool need_rows, bool need_weights, const at::Tensor& status) {
+  no_tangents({&dy, &rows, &weights});
   TORCH_CHECK(dy.is_cuda() && dy.dim() == 2 && dy.is_contiguous() && dy.scalar_type() == at::kBFloat16, "dy must be a contiguous bf16 CUDA tensor [tokens, cols]");
   TORCH_CHECK(rows.is_cuda() && rows.device() == dy.device() && rows.dim() == 2 && rows.is_contiguous() && rows.size(1) == dy.size(1),
               "rows must be a contiguous tensor [num_rows, cols] on dy's device");
@@ -357,6 +367,7 @@ at::Tensor linear_workspace(ag_linear_desc_t& d, const at::Tensor& x, bool backw
 
 std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, int64_t activation,
                                           const OptTensor& residual, bool out_fp32, bool keep_pre, const at::Tensor& status, int64_t timeout_ms) {
+  no_tangents({&x, &weight, get(bias), get(residual)});
   ag_linear_desc_t d = linear_desc(x, weight, activation, status, timeout_ms);
   const at::ScalarType out_type = out_fp32 ? at::kFloat : x.scalar_type();
   d.out_dtype = type_code(out_type, "out");
@@ -392,6 +403,7 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight, int64_t activation,
                                                                const OptTensor& pre, bool need_x, bool need_weight, bool need_bias, bool bias_fp32,
                                                                const at::Tensor& status, int64_t timeout_ms) {
+  no_tangents({&dy, &x, &weight, get(pre)});
   ag_linear_desc_t d = linear_desc(x, weight, activation, status, timeout_ms);
   check_rows(dy, "dy");
   TORCH_CHECK(dy.device() == x.device() && dy.size(0) == d.m && dy.size(1) == d.n && (dy.scalar_type() == x.scalar_type() || dy.scalar_type() == at::kFloat),

@@ -4,7 +4,7 @@ memory are the grouped GEMMs' business: a single dense product would read them a
 
 The kernels are tcgen05 products fed by TMA, so rows of `x` and `weight` start on 16-byte boundaries: k is a multiple of 8.
 Everything runs on the current stream; there is no CPU branch. `linear` is recorded by autograd; `linear_backward` is the same
-gradient as a function of its own, which is the form to capture into a CUDA graph.
+gradient as a function of its own, which is the form to capture into a CUDA graph. Forward-mode derivatives are refused.
 """
 from __future__ import annotations
 
@@ -33,6 +33,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     Sums are fp32, rounded once to the output's type (fp32 outputs, e.g. router logits, are as accurate as an fp32 product of
     the same operands). `return_pre`: also return z = x weight^T + bias in the operands' type, which `linear_backward` needs
     for an activation (None without one). Differentiable with respect to x, weight, bias and residual."""
+    api._refuse_tangents(x, weight, bias, residual)
     act = _activation(activation)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype != x.dtype and out_dtype != torch.float32:
@@ -69,6 +70,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act
 
     dz = dy act'(z) is rounded to the operands' type (as dy is where it is fp32) because the tensor cores take it as an operand;
     dbias sums it before that rounding, in fp32 and in a fixed order."""
+    api._refuse_tangents(dy, x, weight, pre)
     act = _activation(activation)
     bias_dtype = x.dtype if bias_dtype is None else bias_dtype
     if bias_dtype != x.dtype and bias_dtype != torch.float32:

@@ -6,7 +6,8 @@ be exercised by gloo ranks without a GPU; the quantisers, the router and the GEM
 
 `route_topk` and `combine_topk` are differentiable: with gradients enabled, calls whose logits, rows or weights require
 one are recorded for autograd. Their gradients are also functions of their own (`route_topk_backward`,
-`combine_topk_backward`), which is the form to capture into a CUDA graph.
+`combine_topk_backward`), which is the form to capture into a CUDA graph. Forward-mode derivatives exist for `combine_topk` (in plain
+torch); the router refuses them.
 """
 from __future__ import annotations
 
@@ -161,6 +162,8 @@ def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, t
     None = t*top_k + j. Slots with a negative pos (pairs a layout dropped) add nothing. Differentiable with respect to `rows` and
     `weights`; where the CUDA kernels run (contiguous rows, bf16 or fp32, cols a multiple of 8) the gradient is
     `combine_topk_backward`'s: no two slots may name the same row. Elsewhere it is plain torch's."""
+    if api._has_tangent(rows, weights) and _has_combine_kernel(rows):
+        return _combine_plain(rows, pos, weights, tokens, top_k).to(torch.bfloat16)      # the kernels have no forward-mode derivative
     if _has_combine_kernel(rows) and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
     return combine_topk_forward(rows, pos, weights, tokens, top_k)
@@ -205,6 +208,7 @@ def combine_topk_backward(dy: torch.Tensor, rows: torch.Tensor, pos: Optional[to
     dweights[t, j] = <dy[t], rows[pos]> in fp32; drows[pos] = weights[t, j] * dy[t], rounded once, and 0 in rows that no
     slot names. Slots with a pos outside the rows add nothing. With `need_rows` a row may be named by one slot only, as every
     layout here does: a second one sets the status word (`check_status` raises). cols must be a multiple of 8."""
+    api._refuse_tangents(dy, rows, weights)
     w = weights if weights.dtype == torch.float32 and weights.is_contiguous() else weights.to(torch.float32).contiguous()
     return _lib.torch_ops().combine_topk_backward(dy, rows, pos, w, bool(need_rows), bool(need_weights), api._status_word(dy.device))
 
@@ -264,6 +268,7 @@ def route_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias:
     -1 and weight 0; `route_layout` and `combine_topk` skip them. At most 1024 experts, 32 groups, top_k 32.
 
     Differentiable with respect to `logits` through the weights (`route_topk_backward`)."""
+    api._refuse_tangents(logits, bias)
     args = (int(top_k), _named(_SCORING, scoring, "scoring"), bias, int(num_groups), int(top_groups),
             _named(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), float(scale), rows_used)
     if logits.requires_grad and torch.is_grad_enabled():
@@ -275,6 +280,7 @@ def route_topk_backward(dweights: torch.Tensor, topk_ids: torch.Tensor, logits: 
                         scale: float = 1.0) -> torch.Tensor:
     """dlogits [tokens, experts] (type of `logits`) from dweights fp32 [tokens, top_k], the `topk_ids` that `route_topk` chose
     and its arguments. The choice has no gradient; slots with id -1 add nothing."""
+    api._refuse_tangents(dweights, logits)
     return _lib.torch_ops().route_topk_backward(dweights, topk_ids, logits, _named(_SCORING, scoring, "scoring"), bool(renormalize), float(scale))
 
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import asymgemm_b200 as ag
-from asymgemm_b200 import moe_ops
+from asymgemm_b200 import dense_ops, moe_ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -116,7 +116,7 @@ def test_gradient_of_the_combine_at_widths_where_only_the_sum_has_a_kernel(cols,
 LAYOUTS_AT_THE_SHARED_MEMORY_LIMIT = """
 import threading, torch
 import asymgemm_b200 as ag
-from asymgemm_b200 import moe_ops
+from asymgemm_b200 import dense_ops, moe_ops
 
 def check(tokens, experts):
     ids = torch.randint(-1, experts, (tokens, 2), generator=torch.Generator().manual_seed(experts))
@@ -152,3 +152,42 @@ def test_layouts_at_the_limit_of_shared_memory_and_from_several_threads():
     """In a process of its own: 351 experts, whose tables just pass the default limit together with the kernel's own, come first."""
     res = subprocess.run([sys.executable, "-c", LAYOUTS_AT_THE_SHARED_MEMORY_LIMIT], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0 and res.stdout.strip() == "done", res.stdout + res.stderr
+
+
+def test_forward_mode_derivatives_are_refused_or_right():
+    """A tangent is never dropped in silence."""
+    from torch.autograd import forward_ad
+    x, w, g = randn(8, 64, seed=11, dtype=torch.bfloat16), randn(16, 64, seed=12, dtype=torch.bfloat16), randn(8, 16, seed=13, dtype=torch.bfloat16)
+    logits, dw, bias = randn(8, 16, seed=14), randn(8, 2, seed=15), randn(16, seed=16)
+    ids, _ = moe_ops.route_topk(logits, 2)
+    rows, pos, weights = randn(16, 64, seed=17, dtype=torch.bfloat16), torch.randperm(16, device=DEV), torch.rand((8, 2), device=DEV)
+    pos[3] = -1
+    dy = randn(8, 64, seed=18, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: moe_ops.route_topk(dual(logits), 2), lambda: moe_ops.route_topk(logits, 2, bias=dual(bias)),
+                     lambda: moe_ops.route_topk(dual(logits.clone().requires_grad_(True)), 2),
+                     lambda: moe_ops.route_topk_backward(dual(dw), ids, logits), lambda: moe_ops.route_topk_backward(dw, ids, dual(logits)),
+                     lambda: dense_ops.linear(dual(x), w), lambda: dense_ops.linear(x, dual(w)), lambda: dense_ops.linear(x, w, bias=dual(bias)),
+                     lambda: dense_ops.linear(x, w, residual=dual(g)), lambda: dense_ops.linear(dual(x), w.clone().requires_grad_(True)),
+                     lambda: dense_ops.linear(dual(x.view(2, 4, 64)), w), lambda: dense_ops.linear_backward(dual(g), x, w), lambda: dense_ops.linear_backward(g, dual(x), w),
+                     lambda: dense_ops.linear_backward(g, x, w, activation="relu", pre=dual(g)),
+                     lambda: moe_ops.combine_topk_backward(dual(dy), rows, pos, weights), lambda: moe_ops.combine_topk_backward(dy, dual(rows), pos, weights)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        for a, b in ((dual(rows), weights), (rows, dual(weights)), (dual(rows), dual(weights))):
+            y, tangent = forward_ad.unpack_dual(moe_ops.combine_topk(a, pos, b, 8, 2))
+            assert y.dtype == torch.bfloat16
+            live, at = (pos >= 0).view(8, 2, 1), pos.clamp(min=0)
+            r, ws = rows.double()[at].view(8, 2, 64), weights.double().unsqueeze(2)
+            want = (torch.where(live, ws, 0).expand_as(r) * (a is not rows) + torch.where(live, r, 0) * (b is not weights))
+            # three roundings to bf16 at most (the tangents' own, the sum's) and fp32 sums of two
+            assert bool(((tangent.double() - want.sum(1)).abs() <= want.abs().sum(1) * (3 * 2 ** -8)).all())
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: moe_ops.route_topk(t, 2)[1], (logits,), (torch.ones_like(logits),))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: dense_ops.linear(t, w), (x,), (torch.ones_like(x),))
+    # outside of all that the calls are what they were
+    assert torch.equal(moe_ops.route_topk(logits, 2)[0], ids)
