@@ -265,7 +265,8 @@ def route_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias:
     The order is that of exact arithmetic: fp32 scores too close to tell apart are compared in fp64. A NaN or -inf logit or
     bias switches an expert off for the token, a +inf logit counts as the largest finite number. Slots for which no expert is
     left, and all slots of tokens from `rows_used` on (device int32 tensor of one element: a batch padded at its end), get id
-    -1 and weight 0; `route_layout` and `combine_topk` skip them. At most 1024 experts, 32 groups, top_k 32.
+    -1 and weight 0; `route_layout` and `combine_topk` skip them. At most 1024 experts, 32 groups, top_k 32. Ids and weights lie
+    side by side in one allocation, which each of them keeps.
 
     Differentiable with respect to `logits` through the weights (`route_topk_backward`)."""
     api._refuse_tangents(logits, bias)
@@ -302,7 +303,8 @@ class _RouteTopK(torch.autograd.Function):
 
 
 class RouteLayout(NamedTuple):
-    """Tables of the contiguous layout (`route_layout`)."""
+    """Tables of the contiguous layout (`route_layout`). They lie side by side in one allocation (one takes the host less time than
+    five): each keeps the memory of all, and `torch.save` writes all, so clone what outlives the step, e.g. `rows_per_expert`."""
     pair_row: torch.Tensor         # int64 [tokens * top_k]: row of every (token, slot) pair, -1 = none (`pos` of combine_topk)
     row_token: torch.Tensor        # int64 [rows]: token of every row, -1 = padding (`src_rows` of move_rows)
     rows_per_expert: torch.Tensor  # int64 [experts]
@@ -311,7 +313,7 @@ class RouteLayout(NamedTuple):
 
 
 class MaskedRouteLayout(NamedTuple):
-    """Tables of the masked layout (`route_layout_masked`)."""
+    """Tables of the masked layout (`route_layout_masked`); one allocation, as for `RouteLayout`."""
     pair_row: torch.Tensor         # int64 [tokens * top_k]: row in the flattened [experts * max_rows], -1 = none or dropped
     row_token: torch.Tensor        # int64 [experts * max_rows]: token of every row, -1 = unused
     masked_m: torch.Tensor         # int32 [experts]: rows used

@@ -191,3 +191,14 @@ def test_forward_mode_derivatives_are_refused_or_right():
         torch.func.jvp(lambda t: dense_ops.linear(t, w), (x,), (torch.ones_like(x),))
     # outside of all that the calls are what they were
     assert torch.equal(moe_ops.route_topk(logits, 2)[0], ids)
+
+
+def test_tables_of_one_allocation_do_not_overlap():
+    for tokens, experts, k in ((1, 3, 1), (37, 60, 5), (700, 16, 3)):
+        ids, weights = moe_ops.route_topk(randn(tokens, experts, seed=20), k)
+        for tables in ((ids, weights), tuple(moe_ops.route_layout(ids, experts)), tuple(moe_ops.route_layout_masked(ids, experts, 7))):
+            before = [t.clone() for t in tables]
+            for i, t in enumerate(tables):
+                t.fill_(-77)
+                assert all(torch.equal(a, b) for j, (a, b) in enumerate(zip(tables, before)) if j != i)
+                t.copy_(before[i])
