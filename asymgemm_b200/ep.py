@@ -34,10 +34,10 @@ MAX_HISTOGRAM_EXPERTS = 8192      # experts that ag_ep_histogram counts
 @dataclass
 class DispatchState:
     """Everything `combine` needs to send results back and undo the permutations of `dispatch`."""
-    order: Optional[torch.Tensor]  # [T*k] positions of the (token, slot) pairs sorted by expert
+    order: Optional[torch.Tensor]  # positions of the (token, slot) pairs sorted by expert; those without one are last (one rank) or left out
     send_splits: List[int]       # rows sent to each rank
     recv_splits: List[int]       # rows received from each rank
-    dest_rows: Optional[torch.Tensor]  # [R] row of every received row in the padded contiguous layout
+    dest_rows: Optional[torch.Tensor]  # [R] row of every received row in the padded contiguous layout, -1 = none
     rows_per_expert: torch.Tensor  # [experts_per_rank] valid rows of every local expert (device tensor)
     padded_rows: int             # rows allocated for the contiguous layout (upper bound; every expert padded to 128)
     offsets: torch.Tensor        # int32 [2*experts_per_rank] (start, end) pairs; empty experts have start == end
@@ -45,7 +45,37 @@ class DispatchState:
     tokens: int
     top_k: int
     src_token: Optional[torch.Tensor] = None   # one rank only: rows were not gathered yet; received row i is token src_token[i]
-    tables: Optional[moe_ops.RouteLayout] = None   # one rank on a GPU: the layout's tables in place of order, dest_rows, src_token
+    tables: Optional[moe_ops.RouteLayout] = None   # one rank on a GPU: the layout's own tables
+
+
+class _TablesState(DispatchState):
+    """State of one rank on a GPU. The layout kernels need no sort; `order`, `dest_rows` and `src_token` are worked out from their
+    tables each time somebody asks."""
+
+    @property
+    def order(self) -> torch.Tensor:
+        row = self.tables.pair_row
+        return torch.argsort(torch.where(row < 0, self.padded_rows, row), stable=True)
+
+    @property
+    def dest_rows(self) -> torch.Tensor:
+        return self.tables.pair_row.index_select(0, self.order)
+
+    @property
+    def src_token(self) -> torch.Tensor:
+        return torch.div(self.order, self.top_k, rounding_mode="floor")
+
+    @order.setter
+    def order(self, value) -> None:
+        pass
+
+    @dest_rows.setter
+    def dest_rows(self, value) -> None:
+        pass
+
+    @src_token.setter
+    def src_token(self, value) -> None:
+        pass
 
 
 class EPDispatcher:
@@ -166,8 +196,8 @@ class EPDispatcher:
         if self.world == 1 and topk_ids.is_cuda and self.num_experts <= moe_ops.MAX_LAYOUT_EXPERTS and topk_ids.dtype in (torch.int64, torch.int32):
             tables = moe_ops.route_layout(topk_ids.contiguous(), self.num_experts, ALIGN)
             splits = [tokens * top_k]
-            state = DispatchState(None, splits, splits, None, tables.rows_per_expert, tables.row_token.numel(), tables.offsets, tables.experts,
-                                  tokens, top_k, tables=tables)
+            state = _TablesState(None, splits, splits, None, tables.rows_per_expert, tables.row_token.numel(), tables.offsets, tables.experts,
+                                 tokens, top_k, tables=tables)
             return state, rows, tuple(extras)
         if self.world == 1:
             order, send_counts, recv_counts = self.plan(topk_ids)

@@ -188,3 +188,18 @@ def test_ids_outside_the_experts_are_dropped_and_reported_by_the_dispatcher(expe
     with pytest.raises(RuntimeError, match="expert id"):
         ag.check_status()
     ag.check_status()
+
+
+@pytest.mark.parametrize("missing", [0.0, 0.3, 1.0])
+def test_the_state_of_one_gpu_has_the_sort_that_the_cpu_has(missing):
+    tokens, experts, k = 43, 7, 3
+    gen = torch.Generator().manual_seed(80)
+    ids = torch.stack([torch.randperm(experts, generator=gen)[:k] for _ in range(tokens)])
+    ids[torch.rand(ids.shape, generator=gen) < missing] = -1
+    x = torch.randn((tokens, 8), generator=gen)
+    gpu, _, _ = ep.EPDispatcher(experts).dispatch(x.to(DEV), ids.to(DEV))
+    cpu, _, _ = ep.EPDispatcher(experts).dispatch(x, ids)
+    assert isinstance(gpu, ep.DispatchState) and gpu.tables is not None
+    for name in ("order", "dest_rows", "src_token"):
+        assert torch.equal(getattr(gpu, name).cpu(), getattr(cpu, name)), name
+    assert gpu.send_splits == cpu.send_splits and gpu.recv_splits == cpu.recv_splits and gpu.padded_rows == cpu.padded_rows
