@@ -144,16 +144,21 @@ def move_rows_into(out: torch.Tensor, src: torch.Tensor, dst_rows: torch.Tensor)
 
 
 def _has_combine_kernel(rows: torch.Tensor) -> bool:
-    return rows.is_cuda and rows.is_contiguous() and rows.shape[1] % {torch.bfloat16: 8, torch.float32: 4}.get(rows.dtype, 1 << 62) == 0
+    if not rows.is_cuda:
+        return False
+    dtype, cols = rows.dtype, rows.shape[1]
+    return (cols % 8 == 0 if dtype is torch.bfloat16 else dtype is torch.float32 and cols % 4 == 0) and rows.is_contiguous()
 
 
 def _check_combine_tables(rows, pos, weights, pairs: int) -> None:
     """What the kernels read by address: wrong types or too few entries would be read past their end."""
-    if pos is not None and not (pos.dtype == torch.int64 and pos.device == rows.device and pos.is_contiguous() and pos.numel() >= pairs):
+    gpu = rows.get_device()
+    if pos is None:
+        if rows.shape[0] < pairs:
+            raise RuntimeError(f"without pos, rows must hold a row for each of the {pairs} slots")
+    elif pos.dtype is not torch.int64 or pos.get_device() != gpu or not pos.is_contiguous() or pos.numel() < pairs:
         raise RuntimeError(f"pos must be a contiguous int64 tensor of {pairs} entries at least, on the device of rows")
-    if pos is None and rows.shape[0] < pairs:
-        raise RuntimeError(f"without pos, rows must hold a row for each of the {pairs} slots")
-    if weights.device != rows.device or weights.numel() < pairs:
+    if weights.get_device() != gpu or weights.numel() < pairs:
         raise RuntimeError(f"weights must hold {pairs} entries on the device of rows")
 
 
@@ -164,7 +169,7 @@ def combine_topk(rows: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, t
     `combine_topk_backward`'s: no two slots may name the same row. Elsewhere it is plain torch's."""
     if api._has_tangent(rows, weights) and _has_combine_kernel(rows):
         return _combine_plain(rows, pos, weights, tokens, top_k).to(torch.bfloat16)      # the kernels have no forward-mode derivative
-    if _has_combine_kernel(rows) and torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if (rows.requires_grad or weights.requires_grad) and torch.is_grad_enabled() and _has_combine_kernel(rows):
         return _CombineTopK.apply(rows, pos, weights, tokens, top_k)
     return combine_topk_forward(rows, pos, weights, tokens, top_k)
 
@@ -178,12 +183,12 @@ def combine_topk_forward(rows: torch.Tensor, pos: torch.Tensor, weights: torch.T
     if tokens == 0:
         return torch.empty((0, cols), dtype=torch.bfloat16, device=rows.device)
     if pos is not None:
-        rows, pos = _never_empty(rows), pos.reshape(-1)[: tokens * top_k]      # a table may be longer than the batch
+        rows = _never_empty(rows)
     _check_combine_tables(rows, pos, weights, tokens * top_k)
     if rows.dtype == torch.float32 and pos is None:
         pos = torch.arange(tokens * top_k, device=rows.device)
     y = torch.empty((tokens, cols), dtype=torch.bfloat16, device=rows.device)
-    w = weights.to(torch.float32).contiguous()
+    w = weights if weights.dtype is torch.float32 and weights.is_contiguous() else weights.to(torch.float32).contiguous()
     with torch.cuda.device(rows.device):
         combine = _lib.load().ag_combine_topk if rows.dtype == torch.bfloat16 else _lib.load().ag_combine_topk_f32
         _lib.check(combine(rows.data_ptr(), pos.data_ptr() if pos is not None else None, w.data_ptr(), y.data_ptr(), tokens, top_k, cols, _stream(rows)))
