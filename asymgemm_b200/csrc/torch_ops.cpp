@@ -173,6 +173,12 @@ void check_rows(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must have consecutive elements in a row");
   TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), name, " must not have overlapping rows");
 }
+// Rows that lie on one another (an expanded tensor) are copied out; everything else is taken as it is.
+at::Tensor apart(const at::Tensor& t) {
+  const bool expanded = t.dim() == 2 && t.size(0) > 1 && t.stride(0) < t.size(1) && (t.size(1) == 1 || t.stride(1) == 1);
+  return expanded ? t.contiguous() : t;
+}
+OptTensor apart(const OptTensor& t) { return t.has_value() && t->defined() ? OptTensor(apart(*t)) : t; }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 void check_same_device(const OptTensor& t, const char* name, const at::Tensor& a, at::ScalarType type, int64_t numel) {
@@ -182,9 +188,10 @@ void check_same_device(const OptTensor& t, const char* name, const at::Tensor& a
               " elements");
 }
 
-std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits, int64_t top_k, int64_t scoring, const OptTensor& bias, int64_t groups,
+std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits_in, int64_t top_k, int64_t scoring, const OptTensor& bias, int64_t groups,
                                               int64_t top_groups, bool group_max, bool renormalize, double scale, const OptTensor& rows_used) {
-  no_tangents({&logits, get(bias)});
+  no_tangents({&logits_in, get(bias)});
+  const at::Tensor logits = apart(logits_in);
   check_rows(logits, "logits");
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   TORCH_CHECK(experts > 0 && experts <= 1024 && top_k > 0 && top_k <= 32, "route_topk wants 1 .. 1024 experts and top_k 1 .. 32");
@@ -217,9 +224,10 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor& logits, int64_t 
   return {ids, weights};
 }
 
-at::Tensor route_topk_backward(const at::Tensor& dweights, const at::Tensor& ids, const at::Tensor& logits, int64_t scoring, bool renormalize,
+at::Tensor route_topk_backward(const at::Tensor& dweights, const at::Tensor& ids, const at::Tensor& logits_in, int64_t scoring, bool renormalize,
                                double scale) {
-  no_tangents({&dweights, &logits});
+  no_tangents({&dweights, &logits_in});
+  const at::Tensor logits = apart(logits_in);
   check_rows(logits, "logits");
   TORCH_CHECK(ids.dim() == 2 && ids.size(0) == logits.size(0) && ids.size(1) > 0 && ids.size(1) <= 32, "topk_ids must be [tokens, top_k], top_k 1 .. 32");
   TORCH_CHECK(dweights.sizes() == ids.sizes(), "dweights must have the shape of topk_ids");
@@ -365,9 +373,11 @@ at::Tensor linear_workspace(ag_linear_desc_t& d, const at::Tensor& x, bool backw
   return workspace;
 }
 
-std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, int64_t activation,
-                                          const OptTensor& residual, bool out_fp32, bool keep_pre, const at::Tensor& status, int64_t timeout_ms) {
-  no_tangents({&x, &weight, get(bias), get(residual)});
+std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x_in, const at::Tensor& weight_in, const OptTensor& bias, int64_t activation,
+                                          const OptTensor& residual_in, bool out_fp32, bool keep_pre, const at::Tensor& status, int64_t timeout_ms) {
+  no_tangents({&x_in, &weight_in, get(bias), get(residual_in)});
+  const at::Tensor x = apart(x_in), weight = apart(weight_in);
+  const OptTensor residual = apart(residual_in);
   ag_linear_desc_t d = linear_desc(x, weight, activation, status, timeout_ms);
   const at::ScalarType out_type = out_fp32 ? at::kFloat : x.scalar_type();
   d.out_dtype = type_code(out_type, "out");
@@ -400,10 +410,12 @@ std::tuple<at::Tensor, at::Tensor> linear(const at::Tensor& x, const at::Tensor&
   return {y, pre};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight, int64_t activation,
-                                                               const OptTensor& pre, bool need_x, bool need_weight, bool need_bias, bool bias_fp32,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward(const at::Tensor& dy_in, const at::Tensor& x_in, const at::Tensor& weight_in,
+                                                               int64_t activation, const OptTensor& pre_in, bool need_x, bool need_weight, bool need_bias, bool bias_fp32,
                                                                const at::Tensor& status, int64_t timeout_ms) {
-  no_tangents({&dy, &x, &weight, get(pre)});
+  no_tangents({&dy_in, &x_in, &weight_in, get(pre_in)});
+  const at::Tensor dy = apart(dy_in), x = apart(x_in), weight = apart(weight_in);
+  const OptTensor pre = apart(pre_in);
   ag_linear_desc_t d = linear_desc(x, weight, activation, status, timeout_ms);
   check_rows(dy, "dy");
   TORCH_CHECK(dy.device() == x.device() && dy.size(0) == d.m && dy.size(1) == d.n && (dy.scalar_type() == x.scalar_type() || dy.scalar_type() == at::kFloat),

@@ -28,7 +28,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            return_pre: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, Optional[torch.Tensor]]]:
     """y = act(x weight^T + bias) + residual in one kernel: x [..., k], weight [n, k] (both bf16 or both fp16), bias [n] (their type or
     fp32), residual [..., n] (type of the output) -> y [..., n] in `out_dtype`: the operands' type (default) or torch.float32.
-    `activation`: "none", "relu", "gelu" (x Phi(x)) or "silu". x, weight and residual may have any distance between rows.
+    `activation`: "none", "relu", "gelu" (x Phi(x)) or "silu". x, weight and residual may have any distance between rows (rows that
+    lie on one another, as in an expanded tensor, are copied out first).
 
     Sums are fp32, rounded once to the output's type (fp32 outputs, e.g. router logits, are as accurate as an fp32 product of
     the same operands). `return_pre`: also return z = x weight^T + bias in the operands' type, which `linear_backward` needs
@@ -81,8 +82,6 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, act
             raise RuntimeError("x is [..., k] and dy [..., n] with the same leading dimensions")
         x, dy = x.reshape(-1, shape[-1]), dy.reshape(-1, dy.shape[-1])
         pre = pre.reshape(-1, pre.shape[-1]) if pre is not None else None
-    if dy.dim() == 2 and dy.shape[0] > 1 and dy.stride(0) < dy.shape[1]:      # an expanded gradient, e.g. of a sum
-        dy = dy.contiguous()
     dx, dweight, dbias = _lib.torch_ops().linear_backward(dy, x, weight, act, pre, bool(need_x), bool(need_weight), bool(need_bias),
                                                           bias_dtype == torch.float32, api._status_word(x.device), api._state["timeout_ms"])
     return dx.view(shape) if dx is not None else None, dweight, dbias

@@ -202,3 +202,34 @@ def test_tables_of_one_allocation_do_not_overlap():
                 t.fill_(-77)
                 assert all(torch.equal(a, b) for j, (a, b) in enumerate(zip(tables, before)) if j != i)
                 t.copy_(before[i])
+
+
+def test_expanded_operands():
+    """One row or one block of rows under many indices: the strides of the rows are 0 or shorter than a row."""
+    x, w = randn(1, 64, seed=21, dtype=torch.bfloat16), randn(24, 64, seed=22, dtype=torch.bfloat16)
+    r, g = randn(1, 24, seed=23, dtype=torch.bfloat16), randn(10, 24, seed=24, dtype=torch.bfloat16)
+    many = lambda t, *shape: t.expand(*shape)
+    y, pre = dense_ops.linear(many(x, 10, 64), w, activation="silu", residual=many(r, 10, 24), return_pre=True)
+    want, want_pre = dense_ops.linear(x.repeat(10, 1), w, activation="silu", residual=r.repeat(10, 1), return_pre=True)
+    assert torch.equal(y, want) and torch.equal(pre, want_pre)
+    y = dense_ops.linear(many(x, 2, 5, 64), w, residual=many(r, 2, 5, 24))
+    assert torch.equal(y.view(10, 24), dense_ops.linear(x.repeat(10, 1), w, residual=r.repeat(10, 1)))
+    got = dense_ops.linear_backward(g, many(x, 10, 64), w, activation="silu", pre=many(pre[:1], 10, 24))
+    want = dense_ops.linear_backward(g, x.repeat(10, 1), w, activation="silu", pre=pre[:1].repeat(10, 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = dense_ops.linear_backward(many(r, 10, 24), x.repeat(10, 1), w)
+    assert all(torch.equal(a, b) for a, b in zip(got, dense_ops.linear_backward(r.repeat(10, 1), x.repeat(10, 1), w)))
+    assert torch.equal(dense_ops.linear(x, many(w[:1], 9, 64)), dense_ops.linear(x, w[:1].repeat(9, 1)))
+    # broadcast leaves get the sum over their copies
+    leaf, shared = x.clone().requires_grad_(True), r.clone().requires_grad_(True)
+    dx, dr = torch.autograd.grad(dense_ops.linear(many(leaf, 10, 64), w, residual=many(shared, 10, 24)), (leaf, shared), g)
+    rows = dense_ops.linear_backward(g, x.repeat(10, 1), w)[0].double()
+    # ten rows of bf16 numbers summed by torch in fp32 at least, rounded once
+    for a, b in ((dx, rows), (dr, g.double())):
+        assert bool(((a.double() - b.sum(0)).abs() <= b.abs().sum(0) * 16 * 2 ** -24 + b.sum(0).abs() * 2 ** -8).all())
+    logits = randn(1, 16, seed=25)
+    ids, weights = moe_ops.route_topk(many(logits, 7, 16), 3, scoring="sigmoid")
+    want = moe_ops.route_topk(logits.repeat(7, 1), 3, scoring="sigmoid")
+    assert torch.equal(ids, want[0]) and torch.equal(weights, want[1])
+    dw = randn(7, 3, seed=26)
+    assert torch.equal(moe_ops.route_topk_backward(dw, ids, many(logits, 7, 16)), moe_ops.route_topk_backward(dw, ids, logits.repeat(7, 1)))
