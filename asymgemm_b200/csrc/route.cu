@@ -804,7 +804,10 @@ __global__ void __launch_bounds__(128) route_topk_backward_kernel(const RouteGra
     }
   }
   const float l = id >= 0 ? clean(to_float(row[id])) : -INFINITY;
-  if (l == -INFINITY) id = -1;
+  if (l == -INFINITY) {      // switched off: its weight is 0 whatever the gradient asks for
+    id = -1;
+    g = 0.f;
+  }
   float v = 0.f, row_max = 0.f, inv = 0.f, dot = 0.f;
   if (p.renormalize) {
     float top = warp_max_f(l), s = 0.f, rest = 1.f;

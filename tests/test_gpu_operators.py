@@ -233,3 +233,17 @@ def test_expanded_operands():
     assert torch.equal(ids, want[0]) and torch.equal(weights, want[1])
     dw = randn(7, 3, seed=26)
     assert torch.equal(moe_ops.route_topk_backward(dw, ids, many(logits, 7, 16)), moe_ops.route_topk_backward(dw, ids, logits.repeat(7, 1)))
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_router_gradient_leaves_out_switched_off_experts_whatever_their_gradient(scoring, renormalize):
+    logits = randn(4, 40, seed=27)
+    logits[0, 5], logits[1, 7] = -float("inf"), float("nan")
+    ids = torch.tensor([[5, 1, 2], [3, 7, -1], [0, 4, -1], [9, 8, 7]], device=DEV)
+    g = randn(4, 3, seed=28)
+    clean = g.clone()
+    clean[0, 0] = clean[1, 1] = clean[1, 2] = clean[2, 2] = 0
+    g[0, 0], g[1, 1], g[1, 2], g[2, 2] = float("inf"), float("nan"), float("nan"), float("inf")
+    got, want = (moe_ops.route_topk_backward(t, ids, logits, scoring=scoring, renormalize=renormalize) for t in (g, clean))
+    assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
