@@ -98,7 +98,8 @@ struct Slots {
 
 // The same selection in 64 bits: returns the expert chosen i-th on lane i (-1: none left). Every loop is rolled: it runs for a few
 // rows per million, and its size is all that the others see of it (65536 x 256: 53 us inlined so, 57 as a called function, whose
-// calling convention the whole kernel pays for).
+// calling convention the whole kernel pays for). Where every row comes here -- logits that are all equal, as before training, or
+// sigmoids that are saturated -- the same call takes 264 to 293 us.
 template <typename T>
 __device__ __forceinline__ int route_exact(const RouteParams& p, const T* row, int lane) {
   const Slots at(p, p.warp, lane);
@@ -774,8 +775,8 @@ __global__ void __launch_bounds__(128, 8) route_top8_kernel(const RouteParams p)
 //   sigmoid:       dl_i = scale * g_i * s_i * (1 - s_i);
 //   softmax:       dl_j = scale * s_j * ([j chosen] g_j - sum_i s_i g_i), for every expert j.
 // Experts that do not appear get 0, so only the last form reads the whole row; all write it in 16-byte pieces and the few chosen
-// entries over it (65536 x 256 fp32, top 8: 42 us with the entries merged into the pieces before the store, 24 so: 67 MB written, and
-// of the logits a cache line per chosen expert read).
+// entries over it (65536 x 256 fp32, top 8: 42 us with the entries merged into the pieces before the store, 21 to 26 so: 67 MB written,
+// and of the logits a cache line per chosen expert read; the softmax that is not renormalised 42, reading the row three times).
 struct RouteGradParams {
   const void* logits;
   const float* dweights;
@@ -1106,8 +1107,8 @@ void launch_top8(const agb::RouteParams& p, cudaStream_t stream) {
     agb::route_top8_kernel<T, false><<<grid, 128, 0, stream>>>(p);
 }
 // Measured at 65536 x 256 fp32: top 8, softmax 37 us; top 8 of 4 of 8 groups, sigmoid and bias 53 us (550 instructions per row, issue
-// slots 73 % used; reading the logits would take 10 us). Top 16 without groups takes 93 us on a warp
-// per row, where the 53 us case took 104.
+// slots 73 % used; reading the logits would take 10 us). Top 16 takes 89 to 93 us on a warp per
+// row without groups, 128 with sigmoid, bias and 4 of 8 groups; the 53 us case took 104 there.
 template <typename T>
 void launch_route(const agb::RouteParams& p, int sms, cudaStream_t stream) {
   if (p.top_k <= 8) {

@@ -31,8 +31,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     `activation`: "none", "relu", "gelu" (x Phi(x)) or "silu". x, weight and residual may have any distance between rows (rows that
     lie on one another, as in an expanded tensor, are copied out first).
 
-    Sums are fp32, rounded once to the output's type (fp32 outputs, e.g. router logits, are as accurate as an fp32 product of
-    the same operands). `return_pre`: also return z = x weight^T + bias in the operands' type, which `linear_backward` needs
+    Sums are fp32, rounded once to the output's type. (fp32 outputs, e.g. router logits, are off by 4.5e-7 of their norm at k = 7168,
+    where an fp32 product of the same operands is by 1.4e-7 to 9e-7.) `return_pre`: also return z = x weight^T + bias in the operands' type, which `linear_backward` needs
     for an activation (None without one). Differentiable with respect to x, weight, bias and residual."""
     api._refuse_tangents(x, weight, bias, residual)
     act = _activation(activation)

@@ -649,7 +649,8 @@ class ExpertParallelMoE:
         return y
 
     def forward(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
-        """x bf16 [T, hidden] (this rank's tokens), topk_ids int64 [T, k], topk_weights [T, k] -> bf16 [T, hidden]."""
+        """x bf16 [T, hidden] (this rank's tokens), topk_ids int64 [T, k], topk_weights [T, k] -> bf16 [T, hidden]. Ids of -1 mean "no
+        expert": such a pair adds nothing, whatever its weight is. Other ids outside the experts do the same and set the status word."""
         self._mark("start")
         x_q, sfx = moe_ops.quant_rows_fp8(x.contiguous(), pow2_scales=self.ue8m0_scales)
         self._mark("quantise")

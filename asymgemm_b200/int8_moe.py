@@ -145,7 +145,7 @@ class Int8MoELayer:
         self.dispatcher = EPDispatcher(weights.num_experts)
 
     def forward(self, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor) -> torch.Tensor:
-        """x bf16 [T, hidden], topk_ids int64 [T, k], topk_weights fp32 [T, k] -> bf16 [T, hidden]."""
+        """x bf16 [T, hidden], topk_ids int64 [T, k], topk_weights fp32 [T, k] -> bf16 [T, hidden]. Ids of -1 mean "no expert"."""
         from . import api
         w = self.w
         # route rows into the padded contiguous layout first (bf16), then quantise per row there: padding rows are zero,
