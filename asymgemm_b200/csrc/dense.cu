@@ -336,7 +336,11 @@ int run_product(Operand a, Operand b, int64_t k, int type, agb::DenseParams p, v
   p.rows_a = static_cast<int>(a.rows);
   p.rows_b = static_cast<int>(b.rows);
   p.steps = static_cast<int>(steps_of(k));
-  p.chunk_steps = p.out_type == AG_T_FP32 ? agb::kChunkStepsFp32 : agb::kChunkSteps16Bit;
+  // relu's slope turns on the sign of z, which the error of a long run flips for a few in a million -- 1.3e-3 of the gradient, where the
+  // roundings to 16 bits make 2e-4. Runs of 512 flip as few as an fp32 product does (2000 x 2048 x 4096: 6 signs before, 1 now) and cost
+  // 4096 x 4096 x 7168 184 us, where silu in one run takes 177.
+  const bool sign_matters = p.act == agb::ACT_RELU && p.pre != nullptr;
+  p.chunk_steps = p.out_type == AG_T_FP32 || sign_matters ? agb::kChunkStepsFp32 : agb::kChunkSteps16Bit;
   p.tiles_b = static_cast<int>((b.rows + pl.bn - 1) / pl.bn);
   p.swapped = pl.swapped;
   // operand format 0 = fp16, 1 = bf16; bits 15 and 16: A, B are MN-major

@@ -9,7 +9,8 @@
 // at a time into one of two TMEM buffers, and the drain warps add those to fp32 accumulators in registers, rounded to
 // nearest, while it fills the other: the error stays that of one chunk whatever K is. fp32 outputs take chunks of 512
 // terms (1.1e-6 at worst). For outputs that are rounded to 16 bits (half a step is 4.9e-4 or 3.9e-3) chunks of 8192 terms
-// (3.2e-5) change nothing, and the usual product is then one chunk: its epilogue has the whole next tile to run in.
+// (3.2e-5) change nothing, and the usual product is then one chunk: its epilogue has the whole next tile to run in. The exception is
+// a relu whose z is kept for its gradient, which depends on z's sign: chunks of 512.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -420,8 +420,8 @@ int ag_combine_topk_backward(const void* dy_bf16, const void* rows, int32_t rows
  * x [m, k], weight [n, k] bf16 or fp16, rows ldx / ldw elements apart on 16-byte boundaries, k a multiple of 8; bias [n] of their type or
  * fp32, or NULL; y and residual [m, n] of their type or fp32 (out_dtype), rows ldy / ldr apart, residual may be NULL or y itself. `pre`
  * (or NULL) receives z [m, n] in the operands' type, which the gradient of an activation needs. Accumulation in fp32, in runs
- * of terms on the tensor core (512 for fp32 outputs, 8192 for 16-bit ones) joined by rounded fp32 additions; each output is rounded
- * once.
+ * of terms on the tensor core (512 for fp32 outputs and for relu with `pre`, 8192 for other 16-bit ones) joined by rounded fp32
+ * additions; each output is rounded once.
  * Gradients (ag_linear_backward): dz = dy act'(z), rounded to the operands' type for the products; dx [m, k] = dz weight and
  * dweight [n, k] = dz^T x, contiguous, in the operands' type; dbias [n] = column sums of the unrounded dz, in bias_dtype. Any of
  * the three may be NULL. dy [m, n] is of out_dtype, rows lddy apart; the gradient of the residual is dy itself. */

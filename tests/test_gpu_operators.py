@@ -247,3 +247,23 @@ def test_router_gradient_leaves_out_switched_off_experts_whatever_their_gradient
     g[0, 0], g[1, 1], g[1, 2], g[2, 2] = float("inf"), float("nan"), float("nan"), float("inf")
     got, want = (moe_ops.route_topk_backward(t, ids, logits, scoring=scoring, renormalize=renormalize) for t in (g, clean))
     assert bool(torch.isfinite(want).all()) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 7168), (300, 520, 7168), (40, 96, 8192), (2100, 2080, 4096)])
+def test_the_sign_that_the_gradient_of_relu_turns_on(m, n, k, dtype):
+    """Long sums of one sign that the bias takes back to 1e-5 of themselves: z is positive everywhere, by more than what runs of 512
+    terms lose (5.6e-6 of the sum: 40 steps of 2^-23 and one of 2^-24 for each of at most 16 runs) and less than what one run of all does."""
+    x, w = randn(1, k, seed=29, dtype=dtype).abs().expand(m, k).contiguous(), randn(n, k, seed=30, dtype=dtype, scale=0.02).abs()
+    sums = (x[:1].double() @ w.double().t()).view(-1)
+    bias = (-sums * (1 - 1e-5)).float()
+    z = sums + bias.double()
+    assert bool((z > sums * 9.8e-6).all())
+    y, pre = dense_ops.linear(x, w, bias=bias, activation="relu", return_pre=True)
+    assert bool((pre > 0).all()) and bool((y > 0).all())
+    assert bool(((pre.double() - z).abs() <= sums * 6e-6 + z * torch.finfo(dtype).eps).all())
+    dy = torch.ones((m, n), dtype=dtype, device=DEV)
+    db = dense_ops.linear_backward(dy, x, w, activation="relu", pre=pre, need_x=False, need_weight=False, bias_dtype=torch.float32)[2]
+    assert bool((db == m).all())
+    leaf = bias.clone().requires_grad_(True)
+    assert bool((torch.autograd.grad(dense_ops.linear(x, w, bias=leaf, activation="relu").sum(), leaf)[0] == m).all())
