@@ -337,8 +337,8 @@ int run_product(Operand a, Operand b, int64_t k, int type, agb::DenseParams p, v
   p.rows_b = static_cast<int>(b.rows);
   p.steps = static_cast<int>(steps_of(k));
   // relu's slope turns on the sign of z, which the error of a long run flips for a few in a million -- 1.3e-3 of the gradient, where the
-  // roundings to 16 bits make 2e-4. Runs of 512 flip as few as an fp32 product does (2000 x 2048 x 4096: 6 signs before, 1 now) and cost
-  // 4096 x 4096 x 7168 184 us, where silu in one run takes 177.
+  // roundings to 16 bits make 2e-4. Runs of 512 flip as few as an fp32 product does (2000 x 2048 x 4096: 1 sign, 6 in one run of all);
+  // 4096 x 4096 x 7168 takes 184 us so, and silu in one run 177.
   const bool sign_matters = p.act == agb::ACT_RELU && p.pre != nullptr;
   p.chunk_steps = p.out_type == AG_T_FP32 || sign_matters ? agb::kChunkStepsFp32 : agb::kChunkSteps16Bit;
   p.tiles_b = static_cast<int>((b.rows + pl.bn - 1) / pl.bn);
